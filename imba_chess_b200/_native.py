@@ -34,6 +34,7 @@ STATUS_NAMES = {
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_E4M3 = 2  # a KV pool in 8 bits
 # imba_model_desc.flags: SIMT test hooks of a bf16 handle (cross-checks only)
 FLAG_SIMT_GEMM = 1
 FLAG_SIMT_ATTN = 2
@@ -61,6 +62,14 @@ EXPORTED_SYMBOLS = (
     "imba_kv_gather",
     "imba_selftest_wait_timeout",
     "imba_kv_scatter_indexed",
+    "imba_cache_pool_bytes",
+    "imba_append_plan_bytes",
+    "imba_append_plan",
+    "imba_kv_append",
+    "imba_kv_read",
+    "imba_attend_plan_bytes",
+    "imba_attend_plan",
+    "imba_attend",
 )
 
 _P = ctypes.c_void_p
@@ -154,6 +163,39 @@ class StepDesc(ctypes.Structure):
     _fields_ = [(n, _I32) for n in STEP_INT_FIELDS] + [(n, _P) for n in STEP_PTR_FIELDS]
 
 
+class CacheDesc(ctypes.Structure):
+    """A pool's geometry (``imba_cache_desc``)."""
+
+    _fields_ = [(n, _I32) for n in ("num_layers", "num_heads", "attention_dim", "linear_dim", "dtype")]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [(n, _I32) for n in ("rot_dim", "interleaved", "num_axes", "reserved")] + [
+        (n, _P) for n in ("turns", "axis", "positions")]
+
+
+class AppendDesc(ctypes.Structure):
+    _fields_ = ([(n, _I32) for n in ("num_rows", "layer", "src_dtype", "num_q_heads")]
+                + [(n, _P) for n in ("slots", "k", "v", "q", "q_out")]
+                + [(n, ctypes.c_int64 * 3) for n in ("k_stride", "v_stride", "q_stride", "q_out_stride")]
+                + [("rotary", RotaryDesc), ("status", _P)])
+
+
+class AttendDesc(ctypes.Structure):
+    _fields_ = [(n, _I32) for n in ("num_rows", "num_segs", "num_groups", "num_group_pages", "num_extra",
+                                    "num_q_heads")] + [
+        (n, _P) for n in ("seg_group", "seg_row_off", "seg_nrows", "row_perm", "row_vis", "positions",
+                          "group_page_off", "group_pages", "row_extra_off", "extra_slot", "extra_pos", "status")]
+
+
+class AttendArgs(ctypes.Structure):
+    _fields_ = [("layer", _I32), ("dtype", _I32), ("q", _P), ("out", _P), ("q_stride", ctypes.c_int64 * 2),
+                ("out_stride", ctypes.c_int64 * 2), ("scale", ctypes.c_float), ("max_pos", _I32), ("bias", _P)]
+
+
+# in the order of imba_abi_size()
+STRUCTS = (ModelDesc, StepDesc, PoolDesc, CacheDesc, AppendDesc, AttendDesc, AttendArgs)
+
 _lib = None
 _lock = threading.Lock()
 
@@ -175,8 +217,8 @@ def load() -> ctypes.CDLL:
         lib.imba_version.restype = _I32
         lib.imba_abi_size.argtypes = [_I32]
         lib.imba_abi_size.restype = _I32
-        want = (ctypes.sizeof(ModelDesc), ctypes.sizeof(StepDesc), ctypes.sizeof(PoolDesc))
-        got = tuple(int(lib.imba_abi_size(i)) for i in range(3))
+        want = tuple(ctypes.sizeof(c) for c in STRUCTS)
+        got = tuple(int(lib.imba_abi_size(i)) for i in range(len(STRUCTS)))
         if got != want:
             raise NativeLibraryError(
                 f"{LIB_PATH} was built against a different include/imba_b200.h (struct sizes {got}, "
@@ -208,6 +250,20 @@ def load() -> ctypes.CDLL:
         lib.imba_kv_scatter_indexed.restype = _I32
         lib.imba_selftest_wait_timeout.argtypes = [ctypes.c_int64, _P, _P]
         lib.imba_selftest_wait_timeout.restype = _I32
+        cache, pool, rows = ctypes.POINTER(CacheDesc), ctypes.POINTER(PoolDesc), ctypes.POINTER(AttendDesc)
+        for name, args in (("imba_cache_pool_bytes", [cache, ctypes.c_int64]), ("imba_append_plan_bytes", [_I32]),
+                           ("imba_attend_plan_bytes", [cache, rows])):
+            fn = getattr(lib, name)
+            fn.argtypes, fn.restype = args, ctypes.c_size_t
+        for name, args in (
+            ("imba_append_plan", [pool, _I32, _P, _P, ctypes.c_size_t, _P, _P]),
+            ("imba_kv_append", [cache, pool, ctypes.POINTER(AppendDesc), _P, ctypes.c_size_t, _P]),
+            ("imba_kv_read", [cache, pool, _I32, _I32, _P, _I32, _P, _P, _P, _P]),
+            ("imba_attend_plan", [cache, pool, rows, _P, ctypes.c_size_t, _P]),
+            ("imba_attend", [cache, pool, rows, ctypes.POINTER(AttendArgs), _P, ctypes.c_size_t, _P]),
+        ):
+            fn = getattr(lib, name)
+            fn.argtypes, fn.restype = args, _I32
         _lib = lib
         return lib
 

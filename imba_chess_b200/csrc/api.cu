@@ -288,6 +288,10 @@ int32_t imba_abi_size(int32_t which) {
     case 0: return (int32_t)sizeof(imba_model_desc);
     case 1: return (int32_t)sizeof(imba_step_desc);
     case 2: return (int32_t)sizeof(imba_pool_desc);
+    case 3: return (int32_t)sizeof(imba_cache_desc);
+    case 4: return (int32_t)sizeof(imba_append_desc);
+    case 5: return (int32_t)sizeof(imba_attend_desc);
+    case 6: return (int32_t)sizeof(imba_attend_args);
     default: return -1;
   }
 }

@@ -1,0 +1,75 @@
+// Attention over a paged pool in 8 bits (include/imba_b200.h, imba_attend):
+// what the plan pass writes and the kernels read.
+#pragma once
+
+#include "attn_common.cuh"
+#include "cache8.cuh"
+
+namespace imba {
+
+// A tile is up to kTileRows * MT query rows of one segment, flattened with
+// the query heads that share a key / value head (row i, head j of the group:
+// i * share + j).  An item is a tile and a run of its group's pages; a unit
+// is an item and a key / value head.
+constexpr int kTileRows = 16;
+constexpr int kUnitWarps = 8;  // warps of a CTA
+
+struct AttendRow {  // one flattened row of a tile
+  int row;          // -1: none
+  int vis;          // visible tokens of the page list
+  int pos;          // position (bias)
+  int head;         // query head within its group
+};
+struct AttendItem {
+  int tile;
+  int list;    // first entry of the item's pages in group_pages
+  int pages;   // how many
+  int key0;    // position of their first token
+  int part;    // scratch slot of the item's partial result, -1: the tile is not split
+  int splits;  // items of the tile
+  int minvis;  // tokens that every row of the tile sees
+  int index;   // which of them this is (the first takes the rows' extra keys)
+};
+
+struct AttendShape {
+  int share;        // query heads per key / value head
+  int mt;           // 16-row blocks of a tile
+  int warps;        // warps that share a unit: 1 or kUnitWarps
+  int tile_rows;    // kTileRows * mt
+  int max_tiles;
+  int max_items;
+  int max_parts;
+  int min_pages;    // pages of a split item, at least
+  int target;       // items that splitting aims at
+};
+
+// Plan memory, in this order, each part aligned to 256 bytes.
+struct AttendPlan {
+  int* head;             // [0] items
+  int* tile_off;         // [S + 1] first tile of each segment
+  int4* tiles;           // {segment, first flattened row, rows, visible pages}
+  AttendItem* items;
+  AttendRow* rows;       // [max_tiles][tile_rows]
+  int* done;             // [max_tiles][H] items of a split tile that have finished
+  float2* ml;            // [max_parts][H][tile_rows] running maximum and sum
+  float* o;              // [max_parts][H][tile_rows][d_v]
+  size_t bytes;
+};
+
+AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r);
+AttendPlan attend_plan_view(const imba_cache_desc& c, const imba_attend_desc& r, const AttendShape& sh, void* base);
+
+struct AttendArgs {
+  Cache8 cache;
+  AttendPlan plan;
+  AttendShape shape;
+  imba_attend_desc rows;
+  imba_attend_args call;
+};
+
+template <typename T>
+cudaError_t launch_attend8(const imba_cache_desc& c, const AttendArgs& a, cudaStream_t s);
+imba_status_t validate_cache(const imba_cache_desc* c);
+imba_status_t validate_pool(const imba_pool_desc* pool);
+
+}  // namespace imba

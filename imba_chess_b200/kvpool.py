@@ -20,6 +20,15 @@ valid while the game grows, and arena row ``r`` of a turn is token ``r`` of
 that turn's arena sequence - the same row ids the reference mints.
 Sequences are reference-counted; pages return to the pool when the last
 holder releases them.
+
+A pool can also hold its tokens in 8 bits (``dtype=torch.float8_e4m3fn``, half
+of bf16): e4m3 codes with one power-of-two scale for each block of a page's 16
+tokens, head, and K or V.  ``data`` then holds the codes (V's tokens lie in
+pairs, ``[H][8][d_v][2]``) and ``scales`` the scales' exponents, one byte per
+block (0: an empty block).  A block's scale grows with its tokens and never
+shrinks, so pages start afresh when they are handed out: ``alloc`` notes them
+and ``begin_pages`` clears their scales on the stream of the next call that
+writes to the pool.  ``imba_chess_b200.paged`` has the operators on a pool.
 """
 
 from __future__ import annotations
@@ -43,12 +52,27 @@ class KVPool:
                  num_pages: int, dtype: torch.dtype, device: torch.device) -> None:
         if num_pages <= 0:
             raise ValueError("num_pages must be positive")
+        self.num_layers, self.num_heads = int(num_layers), int(num_heads)
+        self.attention_dim, self.linear_dim = int(attention_dim), int(linear_dim)
         self.page_elems = num_layers * num_heads * PAGE * (attention_dim + linear_dim)
         self.num_pages = int(num_pages)
         self.dtype = dtype
         self.device = device
-        self.data = torch.zeros((self.num_pages, self.page_elems), dtype=dtype, device=device)
+        self.scales: torch.Tensor | None = None
+        if dtype == torch.float8_e4m3fn:
+            dims = (32, 64, 96, 128)
+            if attention_dim not in dims or linear_dim not in dims or (
+                    attention_dim != linear_dim and max(attention_dim, linear_dim) > 64):
+                raise ValueError(f"a pool in 8 bits takes head dimensions of {dims} (equal ones above 64), "
+                                 f"got {attention_dim} / {linear_dim}")
+            codes = self.num_pages * self.page_elems
+            memory = torch.zeros(codes + self.num_pages * num_layers * 2 * num_heads, dtype=torch.uint8, device=device)
+            self.data = memory[:codes].view(torch.float8_e4m3fn).view(self.num_pages, self.page_elems)
+            self.scales = memory[codes:].view(self.num_pages, num_layers, 2, num_heads)
+        else:
+            self.data = torch.zeros((self.num_pages, self.page_elems), dtype=dtype, device=device)
         self._free = np.arange(self.num_pages - 1, -1, -1, dtype=np.int64).tolist()
+        self._fresh: list[int] = []  # pages in 8 bits handed out since begin_pages()
         self.desc = _native.PoolDesc(self.data.data_ptr(), self.num_pages)
 
     @property
@@ -57,7 +81,8 @@ class KVPool:
 
     @property
     def page_bytes(self) -> int:
-        return self.page_elems * self.data.element_size()
+        scales = 0 if self.scales is None else 2 * self.num_layers * self.num_heads
+        return self.page_elems * self.data.element_size() + scales
 
     def alloc(self, n: int) -> list[int]:
         if n > len(self._free):
@@ -69,7 +94,27 @@ class KVPool:
         out = self._free[-n:]
         del self._free[-n:]
         out.reverse()
+        if self.scales is not None:
+            self._fresh.extend(out)
         return out
+
+    def begin_pages(self, pages=None) -> None:
+        """Empty the blocks of ``pages`` (default: the pages handed out since
+        the last call) of a pool in 8 bits, on the current stream.  The
+        operators and the model's steps call this; a caller that recycles
+        pages without ``alloc``, or captures a CUDA graph after one, does."""
+        if self.scales is None:
+            return
+        if pages is None:
+            if not self._fresh:
+                return
+            if self.data.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("pages were handed out since the last step: call pool.begin_pages() before the capture")
+            pages, self._fresh = self._fresh, []
+        ids = torch.as_tensor(pages, dtype=torch.int64)
+        if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= self.num_pages):
+            raise ValueError("begin_pages: page id outside the pool")
+        self.scales.index_fill_(0, ids.to(self.device), 0)
 
     def release_pages(self, pages: list[int]) -> None:
         self._free.extend(reversed(pages))

@@ -1,0 +1,318 @@
+"""Operators on a paged KV pool: appending rotated keys and values, and
+attention over a pool held in 8 bits.
+
+A serving program makes the plans once per step and calls the operators for
+every layer::
+
+    pool = KVPool(..., dtype=torch.float8_e4m3fn)
+    rotary = Rotary([10000 ** (-i / 32) for i in range(32)], device=pool.device)
+    rows = AppendPlan(pool, slots)                     # where the step's tokens go
+    sees = AttentionPlan(pool, row_off=..., row_vis=..., page_off=..., pages=..., num_q_heads=32)
+    for layer in range(pool.num_layers):
+        q = kv_append(pool, layer, rows, k, v, rotary=rotary, positions=positions, q=q)
+        out = paged_attention(pool, layer, sees, q)
+
+They stand beside ``B200HSTUChessModel.kv_scatter`` / ``kv_gather`` (rows of a
+model's own pool, as they are); a model with ``kv_dtype=torch.float8_e4m3fn``
+runs its steps on them.  Everything is enqueued on the current stream of the
+pool's device and nothing waits for the device: what only the device can see
+(a slot or a page outside the pool, a row that is not finite) is skipped,
+written to ``pool``'s status word and raised by ``check_status(pool)``.
+
+A plan keeps the tensors it was made from and its scratch: calls on one plan
+must not overlap (two streams, two captured graphs), and the plan's tensors
+hold the step's rows as they were when it was made.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from fractions import Fraction
+
+import torch
+
+from . import _native
+from .kvpool import PAGE, KVPool
+
+_PI = Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
+_DTYPES = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16}
+_POOL_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _native.DTYPE_E4M3}
+_MAX_AXES = 8
+
+
+def _cache(pool: KVPool):
+    """The pool's geometry for the library, and its status word."""
+    got = getattr(pool, "_cache", None)
+    if got is None:
+        if pool.device.type != "cuda" or pool.dtype not in _POOL_DTYPES:
+            raise ValueError(f"the cache operators take a CUDA pool in fp32, bf16 or e4m3, got {pool.dtype} on {pool.device}")
+        if max(pool.attention_dim, pool.linear_dim) > 128:
+            raise ValueError("the cache operators take head dimensions up to 128")
+        desc = _native.CacheDesc(pool.num_layers, pool.num_heads, pool.attention_dim, pool.linear_dim,
+                                 _POOL_DTYPES[pool.dtype])
+        status = torch.zeros(1, dtype=torch.int32, device=pool.device)
+        got = pool._cache = (ctypes.byref(desc), ctypes.byref(pool.desc), status, desc)
+    return got
+
+
+def check_status(pool: KVPool) -> None:
+    """Raise ``ImbaError`` if an operator on this pool reported one (waits for
+    the current stream)."""
+    status = _cache(pool)[2]
+    code = int(status.item())
+    if code != _native.IMBA_OK:
+        status.zero_()
+        raise _native.ImbaError(code, "device-side check")
+
+
+def _stream(pool: KVPool) -> int:
+    return torch.cuda.current_stream(pool.device).cuda_stream
+
+
+def _call(pool: KVPool, what: str, *args) -> None:
+    fn = getattr(_native.load(), what)
+    if torch.cuda.current_device() == pool.data.get_device():
+        code = fn(*args)
+    else:
+        with torch.cuda.device(pool.device):
+            code = fn(*args)
+    if code:
+        _native.check(code, what)
+
+
+def _ints(x, pool: KVPool, what: str, shape: tuple[int, ...] | None = None) -> torch.Tensor:
+    """A contiguous int32 tensor on the pool's device."""
+    t = torch.as_tensor(x)
+    if t.numel() and (t.is_floating_point() or t.is_complex() or t.dtype == torch.bool):
+        raise ValueError(f"{what} must be integers")
+    if t.dtype != torch.int32 and not t.is_cuda and t.numel() and (int(t.max()) > 2**31 - 1 or int(t.min()) < -(2**31)):
+        raise ValueError(f"{what} has values outside int32")
+    if t.is_cuda and t.device != pool.data.device:
+        raise ValueError(f"{what} is on {t.device}, the pool on {pool.data.device}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{what} must have shape {shape}, got {tuple(t.shape)}")
+    return t.to(device=pool.data.device, dtype=torch.int32).contiguous()
+
+
+def _rows(t: torch.Tensor, pool: KVPool, what: str, shape: tuple[int, ...], dtype) -> None:
+    if t.dtype != dtype or t.device != pool.data.device or tuple(t.shape) != shape:
+        raise ValueError(f"{what} must be {dtype} {shape} on {pool.data.device}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+class Rotary:
+    """Rotary positions: pair ``p`` of a head turns by ``positions[axis[p]] *
+    inv_freq[p]`` radians.  ``inv_freq`` has one value per pair, in the order
+    of the pairs; ``layout`` "half" pairs element p with p + len(inv_freq),
+    "interleaved" 2 p with 2 p + 1; the head's other elements pass through.
+    ``axes`` gives each pair's position axis (time, height, width, ...) when
+    tokens have several positions.  Angles are kept as 64-bit fractions of a
+    turn, so they stay right at any position."""
+
+    def __init__(self, inv_freq, *, device, layout: str = "half", axes=None) -> None:
+        freq = [float(f) for f in inv_freq]
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"unknown rotary layout {layout!r}")
+        if not 1 <= len(freq) <= 64 or not all(math.isfinite(f) for f in freq):
+            raise ValueError("inv_freq must hold 1 to 64 finite values")
+        self.num_axes = 1
+        self.axis: torch.Tensor | None = None
+        device = torch.device(device)
+        if axes is not None:
+            axes = [int(a) for a in axes]
+            if len(axes) != len(freq) or min(axes) < 0 or max(axes) >= _MAX_AXES:
+                raise ValueError(f"axes must give each pair an axis in [0, {_MAX_AXES})")
+            self.num_axes = max(axes) + 1
+            self.axis = torch.tensor(axes, dtype=torch.int32, device=device)
+        turns = [round(Fraction(f) / (2 * _PI) * 2**64) % 2**64 for f in freq]
+        self.turns = torch.tensor([t - 2**64 if t >= 2**63 else t for t in turns], dtype=torch.int64, device=device)
+        self.rot_dim = 2 * len(freq)
+        self.layout = layout
+
+
+class AppendPlan:
+    """A step's rows by the pages they go to: row r's token is stored in slot
+    ``slots[r]`` (page * 16 + offset; -1: a padding row).  Of rows with the
+    same slot the last one is stored."""
+
+    def __init__(self, pool: KVPool, slots) -> None:
+        _, desc, status, _ = _cache(pool)
+        self.pool = pool
+        self.slots = _ints(slots, pool, "slots")
+        if self.slots.dim() != 1:
+            raise ValueError("slots must be one-dimensional")
+        self.num_rows = int(self.slots.shape[0])
+        need = int(_native.load().imba_append_plan_bytes(self.num_rows))
+        if need == 0:
+            raise ValueError(f"too many rows for one step: {self.num_rows}")
+        self._plan = torch.empty(need, dtype=torch.uint8, device=pool.data.device)
+        _call(pool, "imba_append_plan", desc, self.num_rows, self.slots.data_ptr(), self._plan.data_ptr(), need,
+              status.data_ptr(), _stream(pool))
+
+
+def kv_append(pool: KVPool, layer: int, plan: AppendPlan, k: torch.Tensor, v: torch.Tensor, *,
+              rotary: Rotary | None = None, positions: torch.Tensor | None = None, q: torch.Tensor | None = None,
+              q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Store a step's keys ``[n, H, d_qk]`` and values ``[n, H, d_v]`` (fp32
+    or bf16, any strides) in one layer of the pool, the keys rotated to
+    ``positions`` (int32 ``[n]``, or ``[n, axes]``) when ``rotary`` is given.
+    ``q`` ``[n, q_heads, d_qk]`` is rotated along and returned (in ``q_out``,
+    which may be ``q``; rows without a slot are left as they were)."""
+    cache, desc, status, _ = _cache(pool)
+    if plan.pool is not pool:
+        raise ValueError("the plan was made for another pool")
+    n, dqk = plan.num_rows, pool.attention_dim
+    dtype = k.dtype
+    if dtype not in _DTYPES:
+        raise ValueError(f"keys and values must be fp32 or bf16, got {dtype}")
+    _rows(k, pool, "k", (n, pool.num_heads, dqk), dtype)
+    _rows(v, pool, "v", (n, pool.num_heads, pool.linear_dim), dtype)
+    a = _native.AppendDesc(n, int(layer), _DTYPES[dtype], 0, plan.slots.data_ptr(), k.data_ptr(), v.data_ptr())
+    a.k_stride[:] = k.stride()
+    a.v_stride[:] = v.stride()
+    if q is not None:
+        if q.dim() != 3 or dqk % 2:
+            raise ValueError("q must be [n, q_heads, d_qk] with an even d_qk")
+        _rows(q, pool, "q", (n, int(q.shape[1]), dqk), dtype)
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        _rows(q_out, pool, "q_out", tuple(q.shape), dtype)
+        a.num_q_heads = int(q.shape[1])
+        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+        a.q_stride[:] = q.stride()
+        a.q_out_stride[:] = q_out.stride()
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if rotary is not None:
+        if rotary.rot_dim > dqk:
+            raise ValueError(f"the rotation takes {rotary.rot_dim} elements, a head has {dqk}")
+        if rotary.turns.device != pool.data.device:
+            raise ValueError("rotary is on another device than the pool")
+        if positions is None:
+            raise ValueError("a rotation needs positions")
+        axes = 1 if positions.dim() == 1 else int(positions.shape[-1])
+        if not rotary.num_axes <= axes <= _MAX_AXES:
+            raise ValueError(f"the rotation takes {rotary.num_axes} positions a row, got {axes}")
+        _rows(positions, pool, "positions", (n,) if positions.dim() == 1 else (n, axes), torch.int32)
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
+        r = a.rotary
+        r.rot_dim, r.interleaved, r.num_axes = rotary.rot_dim, int(rotary.layout == "interleaved"), axes
+        r.turns, r.positions = rotary.turns.data_ptr(), positions.data_ptr()
+        r.axis = None if rotary.axis is None else rotary.axis.data_ptr()
+    a.status = status.data_ptr()
+    pool.begin_pages()
+    if n == 0 or (q is not None and q.numel() == 0):
+        a.num_q_heads = 0
+        a.q = None
+    _call(pool, "imba_kv_append", cache, desc, ctypes.byref(a), plan._plan.data_ptr(), plan._plan.numel(),
+          _stream(pool))
+    return q_out
+
+
+def kv_read(pool: KVPool, layer: int, slots, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The tokens in ``slots`` as dense ``[n, H, d_qk]`` and ``[n, H, d_v]``,
+    in the pool's type; from a pool in 8 bits in bf16, which holds every stored
+    value, or fp32."""
+    cache, desc, status, _ = _cache(pool)
+    dtype = dtype or (torch.bfloat16 if pool.dtype == torch.float8_e4m3fn else pool.dtype)
+    if dtype not in _DTYPES or (pool.dtype != torch.float8_e4m3fn and dtype != pool.dtype):
+        raise ValueError(f"a {pool.dtype} pool is not read as {dtype}")
+    slots = _ints(slots, pool, "slots").reshape(-1)
+    n = int(slots.shape[0])
+    k = torch.empty((n, pool.num_heads, pool.attention_dim), dtype=dtype, device=pool.data.device)
+    v = torch.empty((n, pool.num_heads, pool.linear_dim), dtype=dtype, device=pool.data.device)
+    _call(pool, "imba_kv_read", cache, desc, int(layer), n, slots.data_ptr(), _DTYPES[dtype], k.data_ptr(),
+          v.data_ptr(), status.data_ptr(), _stream(pool))
+    return k, v
+
+
+class AttentionPlan:
+    """What a step's rows see of a pool in 8 bits.
+
+    Rows ``row_off[g] .. row_off[g + 1]`` are of sequence ``g``, whose tokens
+    lie in ``pages[page_off[g] .. page_off[g + 1]]``; row ``r`` sees the first
+    ``row_vis[r]`` of them (a causal row its own token too: position + 1) and
+    then its extra keys, if given: slots ``extra_slot[row_extra_off[r] ..
+    row_extra_off[r + 1]]`` (a suffix chain, the row's own token).
+    ``positions`` (and ``extra_pos``) are for a relative-position bias.  All
+    are int32; on the device they are used as they are."""
+
+    def __init__(self, pool: KVPool, *, row_off, row_vis, page_off, pages, num_q_heads: int, positions=None,
+                 row_extra_off=None, extra_slot=None, extra_pos=None) -> None:
+        cache, desc, status, _ = _cache(pool)
+        if pool.dtype != torch.float8_e4m3fn:
+            raise ValueError(f"attention runs over a pool in 8 bits, got {pool.dtype}")
+        if num_q_heads <= 0 or num_q_heads % pool.num_heads:
+            raise ValueError(f"num_q_heads must be a multiple of the pool's {pool.num_heads} heads")
+        self.pool, self.num_q_heads = pool, int(num_q_heads)
+        row_vis = _ints(row_vis, pool, "row_vis").reshape(-1)
+        self.num_rows = int(row_vis.shape[0])
+        row_off, page_off, pages = (_ints(x, pool, n).reshape(-1) for x, n in (
+            (row_off, "row_off"), (page_off, "page_off"), (pages, "pages")))
+        if row_off.shape[0] < 1 or row_off.shape != page_off.shape:
+            raise ValueError("row_off and page_off must hold one more entry than there are sequences")
+        seqs = int(row_off.shape[0]) - 1
+        keep = {"seg_row_off": row_off, "row_vis": row_vis, "group_page_off": page_off, "group_pages": pages}
+        if positions is not None:
+            keep["positions"] = _ints(positions, pool, "positions", (self.num_rows,))
+        extra = 0
+        if extra_slot is not None:
+            if row_extra_off is None or extra_pos is None:
+                raise ValueError("extra_slot needs row_extra_off and extra_pos")
+            keep["extra_slot"] = _ints(extra_slot, pool, "extra_slot").reshape(-1)
+            extra = int(keep["extra_slot"].shape[0])
+            keep["extra_pos"] = _ints(extra_pos, pool, "extra_pos", (extra,))
+            keep["row_extra_off"] = _ints(row_extra_off, pool, "row_extra_off", (self.num_rows + 1,))
+        self._keep = keep
+        d = self._desc = _native.AttendDesc(self.num_rows, seqs, seqs, int(pages.shape[0]), extra, self.num_q_heads)
+        for name, t in keep.items():
+            setattr(d, name, t.data_ptr())
+        d.status = status.data_ptr()
+        need = int(_native.load().imba_attend_plan_bytes(cache, ctypes.byref(d)))
+        if need == 0:
+            raise ValueError("too many rows or pages for one step")
+        self._plan = torch.empty(need, dtype=torch.uint8, device=pool.data.device)
+        self._args = _native.AttendArgs()
+        self._refs = (ctypes.byref(d), ctypes.byref(self._args), self._plan.data_ptr(), need)
+        _call(pool, "imba_attend_plan", cache, desc, ctypes.byref(d), self._plan.data_ptr(), need, _stream(pool))
+
+
+def paged_attention(pool: KVPool, layer: int, plan: AttentionPlan, q: torch.Tensor, *, scale: float | None = None,
+                    bias: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(scale q . k + bias) v of each row over what its plan says it
+    sees: ``q`` ``[n, q_heads, d_qk]`` (fp32 or bf16; the last dimension
+    contiguous) to ``out`` ``[n, q_heads, d_v]`` of the same type.  ``scale``
+    is 1 / sqrt(d_qk) by default; ``bias`` is fp32 ``[q_heads, 2 max_pos -
+    1]``, its column the key's position less the row's, clamped, plus max_pos
+    - 1.  A row that sees nothing gets zeros."""
+    cache, desc, _, _ = _cache(pool)
+    if plan.pool is not pool:
+        raise ValueError("the plan was made for another pool")
+    n, heads, dtype = plan.num_rows, plan.num_q_heads, q.dtype
+    if dtype not in _DTYPES:
+        raise ValueError(f"queries must be fp32 or bf16, got {dtype}")
+    _rows(q, pool, "q", (n, heads, pool.attention_dim), dtype)
+    if out is None:
+        out = torch.empty((n, heads, pool.linear_dim), dtype=dtype, device=q.device)
+    else:
+        _rows(out, pool, "out", (n, heads, pool.linear_dim), dtype)
+    if q.stride(2) != 1 or out.stride(2) != 1:
+        raise ValueError("the last dimension of q and out must be contiguous")
+    a = plan._args
+    a.layer, a.dtype, a.q, a.out = int(layer), _DTYPES[dtype], q.data_ptr(), out.data_ptr()
+    a.q_stride[:] = q.stride()[:2]
+    a.out_stride[:] = out.stride()[:2]
+    a.scale = pool.attention_dim**-0.5 if scale is None else float(scale)
+    a.bias = None
+    if bias is not None:
+        if bias.dim() != 2 or bias.shape[1] % 2 == 0 or not bias.is_contiguous():
+            raise ValueError("bias must be a contiguous [q_heads, 2 max_pos - 1]")
+        _rows(bias, pool, "bias", (heads, int(bias.shape[1])), torch.float32)
+        if not plan._desc.positions:
+            raise ValueError("a bias needs the plan's positions")
+        a.bias, a.max_pos = bias.data_ptr(), (int(bias.shape[1]) + 1) // 2
+    rows, args, ptr, size = plan._refs
+    _call(pool, "imba_attend", cache, desc, rows, args, ptr, size, _stream(pool))
+    return out

@@ -54,6 +54,7 @@ typedef int32_t imba_status_t;
 
 #define IMBA_DTYPE_F32 0        /* fp32 weights, activations and KV pool          */
 #define IMBA_DTYPE_BF16 1       /* bf16 GEMM operands and KV pool, fp32 residual  */
+#define IMBA_DTYPE_E4M3 2       /* a KV pool in 8 bits (imba_cache_desc.dtype)    */
 
 /* imba_model_desc.flags: test hooks that replace one tensor-core component of
  * a bf16 handle by its fp32-accumulating SIMT kernel, so a test can compare
@@ -189,7 +190,9 @@ typedef struct imba_step_desc {
 /* Library version and the compiled device architecture (e.g. 1000 for sm_100a). */
 IMBA_API int32_t imba_version(void);
 /* sizeof() of the descriptor structs as compiled into the library
- * (0: imba_model_desc, 1: imba_step_desc, 2: imba_pool_desc), so a binding
+ * (0: imba_model_desc, 1: imba_step_desc, 2: imba_pool_desc,
+ * 3: imba_cache_desc, 4: imba_append_desc, 5: imba_attend_desc,
+ * 6: imba_attend_args), so a binding
  * can refuse a library built against a different header. */
 IMBA_API int32_t imba_abi_size(int32_t which);
 IMBA_API int32_t imba_device_arch(void);
@@ -283,6 +286,136 @@ IMBA_API imba_status_t imba_kv_gather(const imba_model* model, const imba_pool_d
                              int32_t layer, int32_t n, const int32_t* slots,
                              void* dense_k, void* dense_v, int32_t* status,
                              void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Cache operators: a paged KV pool used without a model handle, in fp32, bf16
+ * or 8 bits.
+ *
+ * A pool in 8 bits holds e4m3 codes in the page layout above, with one
+ * difference: the tokens of a V block lie in pairs, [H][8][d_v][2] (token 2p
+ * and 2p + 1 of one dimension side by side).  Behind the last page, at byte
+ * num_pages * L * H * 16 * (d_qk + d_v), follow the blocks' scales,
+ * [page][layer][K, V][H], one byte b per block of 16 tokens and head: the
+ * scale is 2^(b - 127), and b = 0 is an empty block.  b is the smallest (at
+ * least 27) for which the block's largest magnitude is at most 448 times the
+ * scale; it never falls while the block lives, and when it grows the codes
+ * that are there are rounded to the new scale (a power of two apart, so only
+ * codes that become subnormal change value).  A page whose blocks are to
+ * start afresh has its scale bytes set to zero first.  The memory starts at
+ * zero, and only these operators write it, so no code is ever a NaN. */
+typedef struct imba_cache_desc {
+  int32_t num_layers;
+  int32_t num_heads;        /* key / value heads                            */
+  int32_t attention_dim;    /* d_qk; in 8 bits both dims are 32, 64, 96 or  */
+  int32_t linear_dim;       /* d_v   128, and equal if one of them is > 64  */
+  int32_t dtype;            /* IMBA_DTYPE_*                                 */
+} imba_cache_desc;
+
+/* Bytes of a pool of num_pages pages (0: a geometry the operators do not
+ * take).  The base is 256-byte aligned. */
+IMBA_API size_t imba_cache_pool_bytes(const imba_cache_desc* cache, int64_t num_pages);
+
+/* The tokens of one step grouped by the page they go to, for
+ * imba_kv_append on a pool in 8 bits: made once per step from the rows'
+ * slots, used for every layer.  Row r goes to slot slots[r]; -1 is a padding
+ * row, which is passed over; other slots outside the pool are skipped and
+ * reported (IMBA_ERR_RANGE).  Of rows with the same slot the last one is
+ * stored.  `plan` is device memory, 256-byte aligned. */
+IMBA_API size_t imba_append_plan_bytes(int32_t num_rows);
+IMBA_API imba_status_t imba_append_plan(const imba_pool_desc* pool, int32_t num_rows, const int32_t* slots,
+                                        void* plan, size_t plan_bytes, int32_t* status, void* stream);
+
+/* Rotary positions: pair p (of rot_dim / 2) of a head turns by
+ * positions[r][axis[p]] * turns[p] / 2^64 whole turns, (a, b) ->
+ * (a cos - b sin, b cos + a sin).  Elements from rot_dim on pass through. */
+typedef struct imba_rotary_desc {
+  int32_t rot_dim;              /* even, <= d_qk; 0: no rotation             */
+  int32_t interleaved;          /* 0: pair p is (p, p + rot_dim / 2); 1: (2p, 2p + 1) */
+  int32_t num_axes;             /* positions per row, 1..8                   */
+  int32_t reserved;
+  const uint64_t* turns;        /* [rot_dim / 2] fraction of a turn per position, times 2^64 */
+  const int32_t* axis;          /* [rot_dim / 2], or NULL: axis 0            */
+  const int32_t* positions;     /* [R, num_axes]                             */
+} imba_rotary_desc;
+
+/* Append rows to one layer, rotated on the way.  Strides (row, head,
+ * element) are in elements.  q may be NULL; q_out may be q itself (with its
+ * strides), else it overlaps no input.  Non-finite elements have no code in
+ * 8 bits: they are stored as zero and reported (IMBA_ERR_RANGE). */
+typedef struct imba_append_desc {
+  int32_t num_rows;
+  int32_t layer;
+  int32_t src_dtype;            /* of k, v, q and q_out: IMBA_DTYPE_F32 / _BF16 */
+  int32_t num_q_heads;          /* 0 when q is NULL                          */
+  const int32_t* slots;         /* [R]                                       */
+  const void* k;                /* [R, H, d_qk]                              */
+  const void* v;                /* [R, H, d_v]                               */
+  const void* q;                /* [R, num_q_heads, d_qk] or NULL            */
+  void* q_out;
+  int64_t k_stride[3], v_stride[3], q_stride[3], q_out_stride[3];
+  imba_rotary_desc rotary;
+  int32_t* status;
+} imba_append_desc;
+/* `plan` (of the same slots) is needed for a pool in 8 bits, else NULL. */
+IMBA_API imba_status_t imba_kv_append(const imba_cache_desc* cache, const imba_pool_desc* pool,
+                                      const imba_append_desc* append, const void* plan, size_t plan_bytes,
+                                      void* stream);
+
+/* Rows of one layer read back: dense [n, H, d_qk] and [n, H, d_v] in
+ * out_dtype (the pool's own type; for a pool in 8 bits bf16, which holds
+ * every stored value, or fp32). */
+IMBA_API imba_status_t imba_kv_read(const imba_cache_desc* cache, const imba_pool_desc* pool, int32_t layer,
+                                    int32_t n, const int32_t* slots, int32_t out_dtype, void* k, void* v,
+                                    int32_t* status, void* stream);
+
+/* Attention over a pool in 8 bits.  Rows come in segments of one sequence
+ * group each; row r sees the first row_vis[r] tokens of its group's page
+ * list, then its extra keys, as in imba_step_desc; a row that sees nothing
+ * gets zeros, and rows of no segment are left as they were.  Query head j
+ * reads key / value head j / (num_q_heads / num_heads). */
+typedef struct imba_attend_desc {
+  int32_t num_rows;
+  int32_t num_segs;
+  int32_t num_groups;
+  int32_t num_group_pages;
+  int32_t num_extra;
+  int32_t num_q_heads;              /* a multiple of the cache's heads               */
+  const int32_t* seg_group;         /* [S], or NULL: segment s is of group s         */
+  const int32_t* seg_row_off;       /* [S], or with seg_nrows NULL [S + 1] offsets   */
+  const int32_t* seg_nrows;         /* [S] or NULL                                   */
+  const int32_t* row_perm;          /* [R] or NULL: row i of the segments' row order */
+  const int32_t* row_vis;           /* [R]                                           */
+  const int32_t* positions;         /* [R] or NULL (the bias needs them)             */
+  const int32_t* group_page_off;    /* [G + 1]                                       */
+  const int32_t* group_pages;
+  const int32_t* row_extra_off;     /* [R + 1] or NULL                               */
+  const int32_t* extra_slot;
+  const int32_t* extra_pos;
+  int32_t* status;
+} imba_attend_desc;
+
+/* Work items of one step, resolved once and read by every layer's
+ * imba_attend; also holds the scratch for sequences that are split, so calls
+ * on one plan must not overlap.  `plan` is device memory, 256-byte aligned. */
+IMBA_API size_t imba_attend_plan_bytes(const imba_cache_desc* cache, const imba_attend_desc* rows);
+IMBA_API imba_status_t imba_attend_plan(const imba_cache_desc* cache, const imba_pool_desc* pool,
+                                        const imba_attend_desc* rows, void* plan, size_t plan_bytes, void* stream);
+
+typedef struct imba_attend_args {
+  int32_t layer;
+  int32_t dtype;                /* of q and out: IMBA_DTYPE_F32 / _BF16                     */
+  const void* q;                /* [R, num_q_heads, d_qk], last dimension contiguous        */
+  void* out;                    /* [R, num_q_heads, d_v], last dimension contiguous         */
+  int64_t q_stride[2];          /* (row, head), elements                                    */
+  int64_t out_stride[2];
+  float scale;                  /* of q . k                                                 */
+  int32_t max_pos;              /* bias has 2 max_pos - 1 columns                           */
+  const float* bias;            /* [num_q_heads, 2 max_pos - 1] or NULL: column             */
+                                /* clamp(key position - positions[r] + max_pos - 1)         */
+} imba_attend_args;
+IMBA_API imba_status_t imba_attend(const imba_cache_desc* cache, const imba_pool_desc* pool,
+                                   const imba_attend_desc* rows, const imba_attend_args* args, void* plan,
+                                   size_t plan_bytes, void* stream);
 
 #ifdef __cplusplus
 }
