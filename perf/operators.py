@@ -239,7 +239,7 @@ def _append_own(s):
     q = paged.kv_append(s["pool"], 0, s["plan"], s["k"], s["v"], rotary=s["rotary"], positions=s["positions"], q=s["q"],
                         q_out=s["q_out"])
     out = {"pages": s["pool"].data, "q": q}
-    return out if s["pool"].scales is None else {**out, "scales": s["pool"].scales.view(torch.float8_e8m0fnu)}
+    return out if s["pool"].scales is None else {**out, "scales": s["pool"].scales[:, 0].view(torch.float8_e8m0fnu)}
 
 
 def _attend_own(s):
