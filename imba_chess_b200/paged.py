@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from fractions import Fraction
 
 import torch
@@ -39,6 +40,11 @@ _PI = Fraction("3.14159265358979323846264338327950288419716939937510582097494459
 _DTYPES = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16}
 _POOL_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _native.DTYPE_E4M3}
 _MAX_AXES = 8
+_FNS: dict = {}
+# imba_append_desc and imba_attend_args as one struct.pack each: these calls run once per layer
+_APPEND = struct.Struct("@4i5P12q4i3PP")
+_ATTEND = struct.Struct("@2i2P4qfiP")
+assert _APPEND.size == ctypes.sizeof(_native.AppendDesc) and _ATTEND.size == ctypes.sizeof(_native.AttendArgs)
 
 
 def _cache(pool: KVPool):
@@ -66,17 +72,21 @@ def check_status(pool: KVPool) -> None:
         raise _native.ImbaError(code, "device-side check")
 
 
-def _stream(pool: KVPool) -> int:
-    return torch.cuda.current_stream(pool.device).cuda_stream
+# the current stream's handle, without a Stream object where torch has the short way
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _call(pool: KVPool, what: str, *args) -> None:
-    fn = getattr(_native.load(), what)
-    if torch.cuda.current_device() == pool.data.get_device():
-        code = fn(*args)
+    """One library call on the current stream of the pool's device."""
+    index = pool.data.get_device()
+    fn = _FNS.get(what) or _FNS.setdefault(what, getattr(_native.load(), what))
+    stream = _raw_stream(index)
+    if torch.cuda.current_device() == index:
+        code = fn(*args, stream)
     else:
-        with torch.cuda.device(pool.device):
-            code = fn(*args)
+        with torch.cuda.device(index):
+            code = fn(*args, stream)
     if code:
         _native.check(code, what)
 
@@ -96,7 +106,7 @@ def _ints(x, pool: KVPool, what: str, shape: tuple[int, ...] | None = None) -> t
 
 
 def _rows(t: torch.Tensor, pool: KVPool, what: str, shape: tuple[int, ...], dtype) -> None:
-    if t.dtype != dtype or t.device != pool.data.device or tuple(t.shape) != shape:
+    if t.dtype != dtype or t.shape != shape or t.get_device() != pool.data.get_device():
         raise ValueError(f"{what} must be {dtype} {shape} on {pool.data.device}, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
@@ -147,8 +157,11 @@ class AppendPlan:
         if need == 0:
             raise ValueError(f"too many rows for one step: {self.num_rows}")
         self._plan = torch.empty(need, dtype=torch.uint8, device=pool.data.device)
+        self._desc = ctypes.create_string_buffer(_APPEND.size)
+        self._refs = (ctypes.cast(self._desc, ctypes.POINTER(_native.AppendDesc)), self._plan.data_ptr(), need,
+                      self.slots.data_ptr(), status.data_ptr())
         _call(pool, "imba_append_plan", desc, self.num_rows, self.slots.data_ptr(), self._plan.data_ptr(), need,
-              status.data_ptr(), _stream(pool))
+              status.data_ptr())
 
 
 def kv_append(pool: KVPool, layer: int, plan: AppendPlan, k: torch.Tensor, v: torch.Tensor, *,
@@ -159,7 +172,7 @@ def kv_append(pool: KVPool, layer: int, plan: AppendPlan, k: torch.Tensor, v: to
     ``positions`` (int32 ``[n]``, or ``[n, axes]``) when ``rotary`` is given.
     ``q`` ``[n, q_heads, d_qk]`` is rotated along and returned (in ``q_out``,
     which may be ``q``; rows without a slot are left as they were)."""
-    cache, desc, status, _ = _cache(pool)
+    cache, desc, _, _ = _cache(pool)
     if plan.pool is not pool:
         raise ValueError("the plan was made for another pool")
     n, dqk = plan.num_rows, pool.attention_dim
@@ -168,22 +181,20 @@ def kv_append(pool: KVPool, layer: int, plan: AppendPlan, k: torch.Tensor, v: to
         raise ValueError(f"keys and values must be fp32 or bf16, got {dtype}")
     _rows(k, pool, "k", (n, pool.num_heads, dqk), dtype)
     _rows(v, pool, "v", (n, pool.num_heads, pool.linear_dim), dtype)
-    a = _native.AppendDesc(n, int(layer), _DTYPES[dtype], 0, plan.slots.data_ptr(), k.data_ptr(), v.data_ptr())
-    a.k_stride[:] = k.stride()
-    a.v_stride[:] = v.stride()
+    q_heads, q_ptrs, q_strides = 0, (0, 0), (0, 0, 0, 0, 0, 0)
     if q is not None:
         if q.dim() != 3 or dqk % 2:
             raise ValueError("q must be [n, q_heads, d_qk] with an even d_qk")
-        _rows(q, pool, "q", (n, int(q.shape[1]), dqk), dtype)
+        _rows(q, pool, "q", (n, q.shape[1], dqk), dtype)
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
-        _rows(q_out, pool, "q_out", tuple(q.shape), dtype)
-        a.num_q_heads = int(q.shape[1])
-        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
-        a.q_stride[:] = q.stride()
-        a.q_out_stride[:] = q_out.stride()
+        else:
+            _rows(q_out, pool, "q_out", q.shape, dtype)
+        if q.numel():
+            q_heads, q_ptrs, q_strides = q.shape[1], (q.data_ptr(), q_out.data_ptr()), (*q.stride(), *q_out.stride())
     elif q_out is not None:
         raise ValueError("q_out without q")
+    turns = (0, 0, 0, 0, 0, 0, 0)
     if rotary is not None:
         if rotary.rot_dim > dqk:
             raise ValueError(f"the rotation takes {rotary.rot_dim} elements, a head has {dqk}")
@@ -191,23 +202,20 @@ def kv_append(pool: KVPool, layer: int, plan: AppendPlan, k: torch.Tensor, v: to
             raise ValueError("rotary is on another device than the pool")
         if positions is None:
             raise ValueError("a rotation needs positions")
-        axes = 1 if positions.dim() == 1 else int(positions.shape[-1])
+        one = positions.dim() == 1
+        axes = 1 if one else int(positions.shape[-1])
         if not rotary.num_axes <= axes <= _MAX_AXES:
             raise ValueError(f"the rotation takes {rotary.num_axes} positions a row, got {axes}")
-        _rows(positions, pool, "positions", (n,) if positions.dim() == 1 else (n, axes), torch.int32)
-        if not positions.is_contiguous():
-            positions = positions.contiguous()
-        r = a.rotary
-        r.rot_dim, r.interleaved, r.num_axes = rotary.rot_dim, int(rotary.layout == "interleaved"), axes
-        r.turns, r.positions = rotary.turns.data_ptr(), positions.data_ptr()
-        r.axis = None if rotary.axis is None else rotary.axis.data_ptr()
-    a.status = status.data_ptr()
-    pool.begin_pages()
-    if n == 0 or (q is not None and q.numel() == 0):
-        a.num_q_heads = 0
-        a.q = None
-    _call(pool, "imba_kv_append", cache, desc, ctypes.byref(a), plan._plan.data_ptr(), plan._plan.numel(),
-          _stream(pool))
+        _rows(positions, pool, "positions", (n,) if one else (n, axes), torch.int32)
+        positions = positions.contiguous()
+        turns = (rotary.rot_dim, rotary.layout == "interleaved", axes, 0, rotary.turns.data_ptr(),
+                 0 if rotary.axis is None else rotary.axis.data_ptr(), positions.data_ptr())
+    if pool._fresh:
+        pool.begin_pages()
+    ref, ptr, size, slots, status = plan._refs
+    _APPEND.pack_into(plan._desc, 0, n, layer, _DTYPES[dtype], q_heads, slots, k.data_ptr(), v.data_ptr(), *q_ptrs,
+                      *k.stride(), *v.stride(), *q_strides, *turns, status)
+    _call(pool, "imba_kv_append", cache, desc, ref, ptr, size)
     return q_out
 
 
@@ -224,7 +232,7 @@ def kv_read(pool: KVPool, layer: int, slots, dtype: torch.dtype | None = None) -
     k = torch.empty((n, pool.num_heads, pool.attention_dim), dtype=dtype, device=pool.data.device)
     v = torch.empty((n, pool.num_heads, pool.linear_dim), dtype=dtype, device=pool.data.device)
     _call(pool, "imba_kv_read", cache, desc, int(layer), n, slots.data_ptr(), _DTYPES[dtype], k.data_ptr(),
-          v.data_ptr(), status.data_ptr(), _stream(pool))
+          v.data_ptr(), status.data_ptr())
     return k, v
 
 
@@ -274,9 +282,10 @@ class AttentionPlan:
         if need == 0:
             raise ValueError("too many rows or pages for one step")
         self._plan = torch.empty(need, dtype=torch.uint8, device=pool.data.device)
-        self._args = _native.AttendArgs()
-        self._refs = (ctypes.byref(d), ctypes.byref(self._args), self._plan.data_ptr(), need)
-        _call(pool, "imba_attend_plan", cache, desc, ctypes.byref(d), self._plan.data_ptr(), need, _stream(pool))
+        self._args = ctypes.create_string_buffer(_ATTEND.size)
+        self._refs = (ctypes.byref(d), ctypes.cast(self._args, ctypes.POINTER(_native.AttendArgs)),
+                      self._plan.data_ptr(), need)
+        _call(pool, "imba_attend_plan", cache, desc, ctypes.byref(d), self._plan.data_ptr(), need)
 
 
 def paged_attention(pool: KVPool, layer: int, plan: AttentionPlan, q: torch.Tensor, *, scale: float | None = None,
@@ -300,19 +309,17 @@ def paged_attention(pool: KVPool, layer: int, plan: AttentionPlan, q: torch.Tens
         _rows(out, pool, "out", (n, heads, pool.linear_dim), dtype)
     if q.stride(2) != 1 or out.stride(2) != 1:
         raise ValueError("the last dimension of q and out must be contiguous")
-    a = plan._args
-    a.layer, a.dtype, a.q, a.out = int(layer), _DTYPES[dtype], q.data_ptr(), out.data_ptr()
-    a.q_stride[:] = q.stride()[:2]
-    a.out_stride[:] = out.stride()[:2]
-    a.scale = pool.attention_dim**-0.5 if scale is None else float(scale)
-    a.bias = None
+    column, max_pos = 0, 0
     if bias is not None:
         if bias.dim() != 2 or bias.shape[1] % 2 == 0 or not bias.is_contiguous():
             raise ValueError("bias must be a contiguous [q_heads, 2 max_pos - 1]")
-        _rows(bias, pool, "bias", (heads, int(bias.shape[1])), torch.float32)
+        _rows(bias, pool, "bias", (heads, bias.shape[1]), torch.float32)
         if not plan._desc.positions:
             raise ValueError("a bias needs the plan's positions")
-        a.bias, a.max_pos = bias.data_ptr(), (int(bias.shape[1]) + 1) // 2
+        column, max_pos = bias.data_ptr(), (bias.shape[1] + 1) // 2
     rows, args, ptr, size = plan._refs
-    _call(pool, "imba_attend", cache, desc, rows, args, ptr, size, _stream(pool))
+    (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
+    _ATTEND.pack_into(plan._args, 0, layer, _DTYPES[dtype], q.data_ptr(), out.data_ptr(), q0, q1, o0, o1,
+                      pool.attention_dim**-0.5 if scale is None else scale, max_pos, column)
+    _call(pool, "imba_attend", cache, desc, rows, args, ptr, size)
     return out
