@@ -7,11 +7,11 @@
 
 namespace imba {
 
-// A tile is up to kTileRows * MT query rows of one segment, flattened with
+// A tile is up to kTileRows * rt query rows of one segment, flattened with
 // the query heads that share a key / value head (row i, head j of the group:
 // i * share + j).  An item is a tile and a run of its group's pages; a unit
 // is an item and a key / value head.
-constexpr int kTileRows = 16;
+constexpr int kTileRows = 8;
 constexpr int kUnitWarps = 8;  // warps of a CTA
 
 struct AttendRow {  // one flattened row of a tile
@@ -33,9 +33,9 @@ struct AttendItem {
 
 struct AttendShape {
   int share;        // query heads per key / value head
-  int mt;           // 16-row blocks of a tile
+  int rt;           // 8-row groups of a tile: 1, 2 or 4
   int warps;        // warps that share a unit: 1 or kUnitWarps
-  int tile_rows;    // kTileRows * mt
+  int tile_rows;    // kTileRows * rt
   int max_tiles;
   int max_items;
   int max_parts;

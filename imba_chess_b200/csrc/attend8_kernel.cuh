@@ -11,14 +11,20 @@
 //
 // Layout.  One warp takes a head's page of 16 tokens at a time, with
 // mma.m16n8k16 on f16 operands and fp32 sums: e4m3 is exact in f16, and the
-// blocks' scales multiply scores and weights, not elements.  A contraction
-// may run over its dimension in any order as long as both operands agree, so
-// the order is chosen for the loads: a lane reads 16 (8 when the head size is
-// no multiple of 64) consecutive bytes of a key, four lanes a key, and these
-// are its B fragments of the next k-steps as they are; V's pairs of tokens
-// are the two halves of a B register, so 16 bytes are eight column tiles'
-// fragments.  No shuffle, no transposition, and what a lane loads it alone
-// reads, so the cp.async ring in shared memory needs no barrier.
+// blocks' scales multiply scores and weights, not elements.  The cache is the
+// 16-row operand, S' = K Q' and O' = V' P', so that a tile is eight query rows
+// and not sixteen: a decode step has few of them, and every instruction but
+// the conversions is per row.  (With the rows as the 16-row operand a step of
+// 1,024 one-token games took 45 us, 32 long sequences 324.)  The weights pass
+// from the result's layout to the operand's by movmatrix.
+//
+// A contraction may run over its dimension in any order as long as both
+// operands agree, so the order is chosen for the loads: a lane reads 16 (8
+// when the head size is no multiple of 64) consecutive bytes of a key, four
+// lanes a key, and these are its fragments of the next k-steps as they are;
+// V's pairs of tokens are the two halves of a register, so 16 bytes are four
+// row tiles' fragments.  No shuffle, and what a lane loads it alone reads, so
+// the cp.async ring in shared memory needs no barrier.
 //
 // Numerics.  A query row is divided by the power of two of its largest
 // element before it becomes f16 (bf16 queries lose nothing above 2^-24 of
@@ -46,6 +52,13 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// An 8 x 8 matrix of f16 from a fragment of its rows to one of its columns.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
@@ -87,13 +100,21 @@ __device__ __forceinline__ void lds(uint32_t src, uint32_t (&w)[B / 4]) {
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(src) : "memory");
 }
 
+// Over the four lanes of a row's query fragment.
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
   return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
 }
-__device__ __forceinline__ float quad_sum(float x) {
-  x += __shfl_xor_sync(0xffffffffu, x, 1);
-  return x + __shfl_xor_sync(0xffffffffu, x, 2);
+// Over the eight lanes that hold a row's keys.
+__device__ __forceinline__ float keys_max(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+__device__ __forceinline__ float keys_sum(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
 }
 
 // The bias in the log2 domain; a finite bias stays finite, so a row whose
@@ -139,28 +160,21 @@ __device__ __forceinline__ void out_store4(T* p, bool vec, const float (&x)[4]) 
   }
 }
 
-// Sizes that follow from the head dimensions.
-template <int DQK, int DV, int MT>
+// Sizes that follow from the head dimensions.  RT: groups of eight rows.
+template <int DQK, int DV, int RT>
 struct Dims {
   static constexpr int VK = DQK % 64 ? 8 : 16, VV = DV % 64 ? 8 : 16;  // bytes of a lane's load
   static constexpr int CK = DQK / 4 / VK, CV = DV / 4 / VV;            // loads per 8 keys / per 4 pairs
-  static constexpr int KS = DQK / 16, NT = DV / 8;                     // k-steps of a score, column tiles of O
-  static constexpr int ROWS = kTileRows * MT;
+  static constexpr int KS = DQK / 16, MV = DV / 16;                    // k-steps of a score, row tiles of O'
+  static constexpr int ROWS = kTileRows * RT;
   static constexpr int STAGE = IMBA_PAGE_TOKENS * (DQK + DV);  // a warp's page
-  static constexpr int MERGE = kUnitWarps * ROWS * (DV * 4 + 8) + ROWS * 4;
-};
-
-// The state of a warp's rows: row 16 i + lane / 4 + 8 r of the tile.
-template <int MT>
-struct RowState {
-  float m[MT][2];  // running maximum (log2 domain)
-  float l[MT][2];  // sum of weights over this lane's keys
+  static constexpr int MERGE = kUnitWarps * ROWS * (DV * 4 + 8) + 16;
 };
 
 // Tile rows joined over the items of a split tile; `nthr` threads from tid on.
-template <typename T, int DQK, int DV, int MT>
+template <typename T, int DQK, int DV, int RT>
 __device__ __forceinline__ void join_items(const AttendArgs& a, const AttendItem& it, int head, int tid, int nthr) {
-  using D = Dims<DQK, DV, MT>;
+  using D = Dims<DQK, DV, RT>;
   const int H = a.cache.H;
   const size_t first = (size_t)(it.part - it.index) * H + head;
   const AttendRow* rows = a.plan.rows + (size_t)it.tile * D::ROWS;
@@ -190,10 +204,112 @@ __device__ __forceinline__ void join_items(const AttendArgs& a, const AttendItem
   }
 }
 
-template <typename T, int DQK, int DV, int MT, int NW, int STAGES>
-__global__ void __launch_bounds__(kUnitWarps * 32, DQK <= 64 && MT == 1 && sizeof(T) == 2 ? 2 : 1)
-    attend8_kernel(AttendArgs a) {
-  using D = Dims<DQK, DV, MT>;
+// A warp's rows and what they have summed up: lane (g, t) = (lane / 4, lane %
+// 4) holds rows 8 i + 2 t + r, i < RT, r < 2, of scores and weights for keys g
+// and g + 8, and of O' for dimensions 4 VV c + VV / 2 g + 0 .. VV / 2 - 1.
+template <int DQK, int DV, int RT, int NP>
+struct Rows {
+  using D = Dims<DQK, DV, RT>;
+  uint32_t q[RT][NP][D::KS][2];  // row 8 i + g: B fragments
+  float fac[RT][2];              // of a raw score, without the block's scale
+  int vis[RT][2], pos[RT][2];
+  const float* bias[RT][2];      // the row's bias, or null
+  float m[RT][2], l[RT][2];      // running maximum (log2 domain), sum over this lane's keys
+  float o[RT][D::MV][4];
+  int vref;                      // scale byte that O is held in units of; 0: none yet
+
+  bool uniform_scales;           // the sixteen keys share their scales (a page)
+
+  // Sixteen keys: from raw scores s (keys g and g + 8; their K scales, V
+  // scale bytes and positions) to weights, as B fragments in p.
+  template <class Mask>
+  __device__ __forceinline__ void weigh(float (&s)[RT][4], const float (&ks)[2], const int (&vb)[2],
+                                        const int (&kpos)[2], int max_pos, bool masked, const Mask& sees,
+                                        uint32_t (&p)[RT][NP][2]) {
+    bool raise = false;
+    float mx[RT][2];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        s[i][r] *= ks[0] * fac[i][r];
+        s[i][2 + r] *= ks[1] * fac[i][r];
+        if (bias[i][r]) {
+          s[i][r] += bias_log2(__ldg(bias[i][r] + bias_index(kpos[0], pos[i][r], max_pos)));
+          s[i][2 + r] += bias_log2(__ldg(bias[i][r] + bias_index(kpos[1], pos[i][r], max_pos)));
+        }
+        if (masked) {
+          if (!sees(i, r, 0)) s[i][r] = -INFINITY;
+          if (!sees(i, r, 1)) s[i][2 + r] = -INFINITY;
+        }
+        mx[i][r] = fmaxf(s[i][r], s[i][2 + r]);
+        raise |= mx[i][r] > m[i][r] + kSlack;
+      }
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float now = fmaxf(m[i][r], keys_max(mx[i][r]));
+          const float w = weight_of(m[i][r], now);
+          m[i][r] = now;
+          l[i][r] *= w;
+#pragma unroll
+          for (int j = 0; j < D::MV; ++j) {
+            o[i][j][r] *= w;
+            o[i][j][2 + r] *= w;
+          }
+        }
+    }
+    // V's scales as ratios to vref, which follows them.
+    float ratio[2] = {1.f, 1.f};
+    int top = max(vb[0], vb[1]), low = min(vb[0] ? vb[0] : 255, vb[1] ? vb[1] : 255);
+    if (!uniform_scales) {
+      top = __reduce_max_sync(0xffffffffu, top);
+      low = __reduce_min_sync(0xffffffffu, low);
+    }
+    if (top) {
+      if (vref == 0) vref = top;
+      if (top - vref > kVWindow || vref - low > kVWindow) {
+        const int now = max(top, vref - 60);
+        const float f = vref - now < -126 ? 0.f : __uint_as_float((uint32_t)(127 + vref - now) << 23);
+        vref = now;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < D::MV; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][j][e] *= f;
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        if (vb[n]) ratio[n] = vb[n] - vref < -126 ? 0.f : __uint_as_float((uint32_t)(127 + vb[n] - vref) << 23);
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      float w[4];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float ref = m[i][r] == -INFINITY ? 0.f : m[i][r] - kShift;
+        w[r] = exp2_approx(s[i][r] - ref);
+        w[2 + r] = exp2_approx(s[i][2 + r] - ref);
+        l[i][r] += w[r] + w[2 + r];
+      }
+      uint32_t lo[NP], hi[NP];
+      split_h2<NP>(w[0] * ratio[0], w[1] * ratio[0], lo);
+      split_h2<NP>(w[2] * ratio[1], w[3] * ratio[1], hi);
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        p[i][n][0] = transpose8(lo[n]);
+        p[i][n][1] = transpose8(hi[n]);
+      }
+    }
+  }
+};
+
+template <typename T, int DQK, int DV, int RT, int NW, int STAGES, int CTAS>
+__global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendArgs a) {
+  using D = Dims<DQK, DV, RT>;
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   extern __shared__ __align__(16) uint8_t smem[];
   pdl_wait();
@@ -205,7 +321,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, DQK <= 64 && MT == 1 && sizeo
   const int item_id = (int)(unit / H), head = (int)(unit % H);
   if (item_id >= a.plan.head[0]) return;
   const AttendItem it = a.plan.items[item_id];
-  const AttendRow* tile = a.plan.rows + (size_t)it.tile * D::ROWS;
+  const int4* tile = reinterpret_cast<const int4*>(a.plan.rows + (size_t)it.tile * D::ROWS);
 
   // This warp's pages: list entries sub, sub + NW, ... of the item, 32 at a
   // time in the lanes (id and the two scale bytes), the next 32 in flight.
@@ -222,16 +338,29 @@ __global__ void __launch_bounds__(kUnitWarps * 32, DQK <= 64 && MT == 1 && sizeo
     const uint8_t* s = a.cache.scales + id * a.cache.scale_stride + head;
     return s[0] | s[H] << 8;
   };
-  int ids = page_id(lane), ids_next = page_id(32 + lane);
+  int ids = page_id(lane), ids_next = npages > 32 ? page_id(32 + lane) : -1;
 
-  AttendRow rows[MT][2];
+  Rows<DQK, DV, RT, NP> st;
+  int4 qrow[RT];  // the rows whose query fragments this lane holds
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int i = 0; i < RT; ++i) {
+    qrow[i] = __ldg(tile + 8 * i + g);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int4 u = __ldg(reinterpret_cast<const int4*>(tile + 16 * i + g + 8 * r));
-      rows[i][r] = AttendRow{u.x, u.y, u.z, u.w};
+      const int4 u = __ldg(tile + 8 * i + 2 * t + r);
+      st.vis[i][r] = u.y;
+      st.pos[i][r] = u.z;
+      st.bias[i][r] = a.call.bias && u.x >= 0
+                          ? a.call.bias + (int64_t)(head * a.shape.share + u.w) * (2 * a.call.max_pos - 1)
+                          : nullptr;
+      st.m[i][r] = -INFINITY;
+      st.l[i][r] = 0.f;
     }
+#pragma unroll
+    for (int j = 0; j < D::MV; ++j) st.o[i][j][0] = st.o[i][j][1] = st.o[i][j][2] = st.o[i][j][3] = 0.f;
+  }
+  st.vref = 0;
+  st.uniform_scales = true;
   int scs = page_scales(ids), scs_next = page_scales(ids_next);
   if (__any_sync(0xffffffffu, ids == -2 || ids_next == -2) && lane == 0) report(a.rows.status, IMBA_ERR_RANGE);
 
@@ -260,54 +389,42 @@ __global__ void __launch_bounds__(kUnitWarps * 32, DQK <= 64 && MT == 1 && sizeo
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) issue(i, ids);
 
-  // Queries: f16 A fragments of each row over its power of two.
-  uint32_t qa[MT][NP][D::KS][4];
-  float fac[MT][2];
+  // Queries: f16 B fragments of each row over its power of two.
   const bool qvec = a.call.q_stride[0] % 4 == 0 && a.call.q_stride[1] % 4 == 0 &&
                     (reinterpret_cast<uintptr_t>(a.call.q) & (4 * sizeof(T) - 1)) == 0;
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int i = 0; i < RT; ++i) {
+    const T* q = static_cast<const T*>(a.call.q) + qrow[i].x * a.call.q_stride[0] +
+                 (int64_t)(head * a.shape.share + qrow[i].w) * a.call.q_stride[1];
+    float x[D::KS][4], amax = 0.f;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const AttendRow& row = rows[i][r];
-      const T* q = static_cast<const T*>(a.call.q) + row.row * a.call.q_stride[0] +
-                   (int64_t)(head * a.shape.share + row.head) * a.call.q_stride[1];
-      float x[D::KS][4], amax = 0.f;
+    for (int s = 0; s < D::KS; ++s) {
+      x[s][0] = x[s][1] = x[s][2] = x[s][3] = 0.f;
+      if (qrow[i].x >= 0) q_load4(q + s / (D::VK / 4) * 4 * D::VK + t * D::VK + s % (D::VK / 4) * 4, qvec, x[s]);
+    }
 #pragma unroll
-      for (int s = 0; s < D::KS; ++s) {
-        x[s][0] = x[s][1] = x[s][2] = x[s][3] = 0.f;
-        if (row.row >= 0) q_load4(q + s / (D::VK / 4) * 4 * D::VK + t * D::VK + s % (D::VK / 4) * 4, qvec, x[s]);
+    for (int s = 0; s < D::KS; ++s)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fabsf(x[s][j]));
-      }
-      amax = quad_max(amax);
-      const int ex = (int)(__float_as_uint(amax) >> 23);  // 0 for a zero row, 255 for an infinite one
-      const int e = ex == 0 || ex == 255 ? 0 : min(ex - 127, 126);
-      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      fac[i][r] = __uint_as_float((uint32_t)(127 + e) << 23) * a.call.scale * kLog2e;
+      for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fabsf(x[s][j]));
+    amax = quad_max(amax);
+    const int ex = (int)(__float_as_uint(amax) >> 23);  // 0 for a zero row, 255 for an infinite one
+    const int e = ex == 0 || ex == 255 ? 0 : min(ex - 127, 126);
+    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+    const float f = __uint_as_float((uint32_t)(127 + e) << 23) * a.call.scale * kLog2e;
+    st.fac[i][0] = __shfl_sync(0xffffffffu, f, 8 * t);
+    st.fac[i][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll
-      for (int s = 0; s < D::KS; ++s) {
-        uint32_t lo[NP], hi[NP];
-        split_h2<NP>(x[s][0] * down, x[s][1] * down, lo);
-        split_h2<NP>(x[s][2] * down, x[s][3] * down, hi);
+    for (int s = 0; s < D::KS; ++s) {
+      uint32_t lo[NP], hi[NP];
+      split_h2<NP>(x[s][0] * down, x[s][1] * down, lo);
+      split_h2<NP>(x[s][2] * down, x[s][3] * down, hi);
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          qa[i][p][s][r] = lo[p];
-          qa[i][p][s][2 + r] = hi[p];
-        }
+      for (int p = 0; p < NP; ++p) {
+        st.q[i][p][s][0] = lo[p];
+        st.q[i][p][s][1] = hi[p];
       }
     }
-
-  RowState<MT> st;
-  float o[MT][D::NT][4];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    st.m[i][0] = st.m[i][1] = -INFINITY;
-    st.l[i][0] = st.l[i][1] = 0.f;
-#pragma unroll
-    for (int j = 0; j < D::NT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
   }
-  int vref = 0;  // scale byte that O is held in units of; 0: none yet
 
   for (int i = 0; i < npages; ++i) {
     if (i && (i & 31) == 0) {
@@ -327,243 +444,204 @@ __global__ void __launch_bounds__(kUnitWarps * 32, DQK <= 64 && MT == 1 && sizeo
     }
     const uint32_t src = ring + i % STAGES * D::STAGE;
     const int key0 = it.key0 + (sub + i * NW) * IMBA_PAGE_TOKENS;
-    const float ks = scale_of(sc & 255);
-    const int vb = sc >> 8;
 
-    // Scores of 16 keys.
-    float s[MT][2][4];
+    float s[RT][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int r = 0; r < RT; ++r) s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.f;
 #pragma unroll
-      for (int n = 0; n < 2; ++n) s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.f;
+    for (int c = 0; c < D::CK; ++c) {
+      uint32_t w0[D::VK / 4], w1[D::VK / 4];
+      lds<D::VK>(src + (c * 32 + lane) * D::VK, w0);
+      lds<D::VK>(src + ((D::CK + c) * 32 + lane) * D::VK, w1);
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+      for (int j = 0; j < D::VK / 4; ++j) {
+        const uint32_t ka[4] = {e4m3x2_to_h2(w0[j]), e4m3x2_to_h2(w1[j]), e4m3x2_to_h2(w0[j] >> 16),
+                                e4m3x2_to_h2(w1[j] >> 16)};
 #pragma unroll
-      for (int c = 0; c < D::CK; ++c) {
-        uint32_t w[D::VK / 4];
-        lds<D::VK>(src + ((n * D::CK + c) * 32 + lane) * D::VK, w);
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int j = 0; j < D::VK / 4; ++j) {
-          const uint32_t b0 = e4m3x2_to_h2(w[j]), b1 = e4m3x2_to_h2(w[j] >> 16);
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int p = 0; p < NP; ++p) mma_f16(s[m][n], qa[m][p][c * (D::VK / 4) + j], b0, b1);
-        }
+          for (int p = 0; p < NP; ++p)
+            mma_f16(s[r], ka, st.q[r][p][c * (D::VK / 4) + j][0], st.q[r][p][c * (D::VK / 4) + j][1]);
       }
+    }
 
-    // log2-domain scores; the keys a row does not see are -inf.
-    const bool whole = id >= 0 && key0 + IMBA_PAGE_TOKENS <= it.minvis;
-    bool raise = false;
-    float mx[MT][2];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float f = ks * fac[m][r];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) s[m][n][2 * r + j] *= f;
-        if (a.call.bias && rows[m][r].row >= 0) {
-          const float* b =
-              a.call.bias + (int64_t)(head * a.shape.share + rows[m][r].head) * (2 * a.call.max_pos - 1);
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              s[m][n][2 * r + j] +=
-                  bias_log2(__ldg(b + bias_index(key0 + n * 8 + 2 * t + j, rows[m][r].pos, a.call.max_pos)));
-        }
-        if (!whole) {
-          const int vis = id >= 0 ? rows[m][r].vis - key0 : 0;
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              if (n * 8 + 2 * t + j >= vis) s[m][n][2 * r + j] = -INFINITY;
-        }
-        mx[m][r] = fmaxf(fmaxf(s[m][0][2 * r], s[m][0][2 * r + 1]), fmaxf(s[m][1][2 * r], s[m][1][2 * r + 1]));
-        raise |= mx[m][r] > st.m[m][r] + kSlack;
-      }
-    if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float now = fmaxf(st.m[m][r], quad_max(mx[m][r]));
-          const float w = weight_of(st.m[m][r], now);
-          st.m[m][r] = now;
-          st.l[m][r] *= w;
-#pragma unroll
-          for (int j = 0; j < D::NT; ++j) {
-            o[m][j][2 * r] *= w;
-            o[m][j][2 * r + 1] *= w;
-          }
-        }
-    }
-    // V's scale as a ratio to vref.
-    float ratio = 1.f;
-    if (vb) {
-      if (vref == 0) vref = vb;
-      if (abs(vb - vref) > kVWindow) {
-        const int now = max(vb, vref - 60);
-        const float f = vref - now < -126 ? 0.f : __uint_as_float((uint32_t)(127 + vref - now) << 23);
-        vref = now;
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int j = 0; j < D::NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[m][j][e] *= f;
-      }
-      ratio = vb - vref < -126 ? 0.f : __uint_as_float((uint32_t)(127 + vb - vref) << 23);
-    }
-    uint32_t pa[MT][NP][4];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float ref = st.m[m][r] == -INFINITY ? 0.f : st.m[m][r] - kShift;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float p0 = exp2_approx(s[m][n][2 * r] - ref), p1 = exp2_approx(s[m][n][2 * r + 1] - ref);
-          st.l[m][r] += p0 + p1;
-          uint32_t h[NP];
-          split_h2<NP>(p0 * ratio, p1 * ratio, h);
-#pragma unroll
-          for (int p = 0; p < NP; ++p) pa[m][p][2 * n + r] = h[p];
-        }
-      }
+    const float ks[2] = {scale_of(sc & 255), scale_of(sc & 255)};
+    const int vb[2] = {sc >> 8, sc >> 8}, kpos[2] = {key0 + g, key0 + g + 8};
+    uint32_t pb[RT][NP][2];
+    st.weigh(s, ks, vb, kpos, a.call.max_pos, id < 0 || key0 + IMBA_PAGE_TOKENS > it.minvis,
+             [&](int r, int e, int n) { return id >= 0 && kpos[n] < st.vis[r][e]; }, pb);
 #pragma unroll
     for (int c = 0; c < D::CV; ++c) {
       uint32_t w0[D::VV / 4], w1[D::VV / 4];
       lds<D::VV>(src + IMBA_PAGE_TOKENS * DQK + (c * 32 + lane) * D::VV, w0);
       lds<D::VV>(src + IMBA_PAGE_TOKENS * DQK + ((D::CV + c) * 32 + lane) * D::VV, w1);
 #pragma unroll
-      for (int j = 0; j < D::VV / 2; ++j) {
-        const uint32_t b0 = e4m3x2_to_h2(w0[j / 2] >> (16 * (j % 2)));
-        const uint32_t b1 = e4m3x2_to_h2(w1[j / 2] >> (16 * (j % 2)));
+      for (int j = 0; j < D::VV / 4; ++j) {
+        const uint32_t va[4] = {e4m3x2_to_h2(w0[j]), e4m3x2_to_h2(w0[j] >> 16), e4m3x2_to_h2(w1[j]),
+                                e4m3x2_to_h2(w1[j] >> 16)};
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-          for (int p = 0; p < NP; ++p) mma_f16(o[m][c * (D::VV / 2) + j], pa[m][p], b0, b1);
+          for (int p = 0; p < NP; ++p) mma_f16(st.o[r][c * (D::VV / 4) + j], va, pb[r][p][0], pb[r][p][1]);
       }
     }
   }
 
-  // The rows' extra keys, one at a time: four lanes share a row, each with
-  // the dimensions that its fragments hold.
+  // The rows' extra keys, sixteen of the tile's at a time: each is seen by
+  // its own row alone, and has its own block's scales.
   if (a.rows.num_extra > 0 && it.index == 0 && sub == 0) {
     const int64_t slots = a.cache.num_pages * IMBA_PAGE_TOKENS;
-    if (vref == 0) vref = 127;
-    const float unref = __uint_as_float((uint32_t)(254 - vref) << 23);
+    int e0 = 0, n = 0;  // lane = row of the tile
+    if (lane < D::ROWS) {
+      const int row = __ldg(tile + lane).x;
+      if (row >= 0) {
+        e0 = a.rows.row_extra_off[row];
+        const int e1 = a.rows.row_extra_off[row + 1];
+        if (e0 < 0 || e1 < e0 || e1 > a.rows.num_extra)
+          report(a.rows.status, IMBA_ERR_RANGE);
+        else
+          n = e1 - e0;
+      }
+    }
+    int upto = n;  // extras of the rows up to this one
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int o = 1; o < 32; o *= 2) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    const int total = __shfl_sync(0xffffffffu, upto, 31);
+    st.uniform_scales = false;
+    for (int x0 = 0; x0 < total; x0 += 16) {
+      // Lane x holds key x0 + x: its row, slot, position and scales.
+      int owner = 0, slot = -1, kp = 0, sc = 0;
+      {
+        const int x = x0 + lane;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const AttendRow row = rows[m][r];
-        int e0 = 0, e1 = 0;
-        if (row.row >= 0) {
-          e0 = a.rows.row_extra_off[row.row];
-          e1 = a.rows.row_extra_off[row.row + 1];
-          if (e0 < 0 || e1 < e0 || e1 > a.rows.num_extra) {
-            report(a.rows.status, IMBA_ERR_RANGE);
-            e0 = e1 = 0;
-          }
+        for (int step = 16; step; step /= 2) {
+          const int y = __shfl_sync(0xffffffffu, upto, owner + step - 1);
+          if (y <= x) owner += step;
         }
-        const int most = __reduce_max_sync(0xffffffffu, e1 - e0);
-        for (int x = 0; x < most; ++x) {
-          int64_t slot = -1;
-          float b = 0.f;
-          if (e0 + x < e1) {
-            slot = a.rows.extra_slot[e0 + x];
-            if (slot < 0 || slot >= slots) {
-              report(a.rows.status, IMBA_ERR_RANGE);
-              slot = -1;
-            }
-            if (a.call.bias)
-              b = bias_log2(a.call.bias[(int64_t)(head * a.shape.share + row.head) * (2 * a.call.max_pos - 1) +
-                                        bias_index(a.rows.extra_pos[e0 + x], row.pos, a.call.max_pos)]);
+        const int past = __shfl_sync(0xffffffffu, upto - n, owner & 31);
+        const int base = __shfl_sync(0xffffffffu, e0, owner & 31);
+        if (lane < 16 && x < total) {
+          slot = a.rows.extra_slot[base + x - past];
+          kp = a.rows.extra_pos[base + x - past];
+          if (slot < 0 || slot >= slots) {
+            report(a.rows.status, IMBA_ERR_RANGE);
+            slot = -1;
+          } else {
+            sc = page_scales(slot / IMBA_PAGE_TOKENS);
           }
-          const int64_t page = max(slot, (int64_t)0) / IMBA_PAGE_TOKENS;
-          const int tok = (int)(max(slot, (int64_t)0) % IMBA_PAGE_TOKENS);
-          const int sc = page_scales((int)page);
-          const uint8_t* k = head_k + page * a.cache.page_stride;
-          float dot = 0.f;
-#pragma unroll
-          for (int c = 0; c < D::CK; ++c)
-#pragma unroll
-            for (int j = 0; j < D::VK / 4; ++j) {
-              const uint32_t w = *reinterpret_cast<const uint32_t*>(k + tok * DQK + c * 4 * D::VK + t * D::VK + 4 * j);
-              const float2 k0 = e4m3x2_to_f2(w), k1 = e4m3x2_to_f2(w >> 16);
-#pragma unroll
-              for (int p = 0; p < NP; ++p) {
-                const float2 q0 = unpack_h2(qa[m][p][c * (D::VK / 4) + j][r]);
-                const float2 q1 = unpack_h2(qa[m][p][c * (D::VK / 4) + j][2 + r]);
-                dot = fmaf(q0.x, k0.x, fmaf(q0.y, k0.y, fmaf(q1.x, k1.x, fmaf(q1.y, k1.y, dot))));
-              }
-            }
-          dot = quad_sum(dot);
-          const float sx = slot < 0 ? -INFINITY : dot * scale_of(sc & 255) * fac[m][r] + b;
-          const float now = fmaxf(st.m[m][r], sx);
-          const float w = weight_of(st.m[m][r], now);
-          const float p = now == -INFINITY && sx == sx ? 0.f : exp2_approx(sx - (now - kShift));
-          st.m[m][r] = now;
-          st.l[m][r] = st.l[m][r] * w + (t == 0 ? p : 0.f);  // summed over the quad at the end
-          const float pv = p * (scale_of(sc >> 8) * unref);
-          const uint8_t* v = k + v_from_k;
-#pragma unroll
-          for (int c = 0; c < D::CV; ++c)
-#pragma unroll
-            for (int j = 0; j < D::VV / 2; ++j) {
-              // column tile c, j: dimensions 4 VV c + VV t + j and that + VV / 2
-              const int e = c * 4 * D::VV + t * D::VV + j;
-              float* od = o[m][c * (D::VV / 2) + j] + 2 * r;
-              od[0] = fmaf(pv, e4m3x2_to_f2(v[v8_off(tok, e, DV)]).x, od[0] * w);
-              od[1] = fmaf(pv, e4m3x2_to_f2(v[v8_off(tok, e + D::VV / 2, DV)]).x, od[1] * w);
-            }
         }
       }
+      int kslot[2], kown[2], kpos[2], vb[2];
+      float ks[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        kslot[k] = __shfl_sync(0xffffffffu, slot, g + 8 * k);
+        kown[k] = __shfl_sync(0xffffffffu, owner, g + 8 * k);
+        kpos[k] = __shfl_sync(0xffffffffu, kp, g + 8 * k);
+        const int both = __shfl_sync(0xffffffffu, sc, g + 8 * k);
+        ks[k] = scale_of(both & 255);
+        vb[k] = both >> 8;
+      }
+      int vslot[4];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+      for (int k = 0; k < 4; ++k) vslot[k] = max(__shfl_sync(0xffffffffu, slot, 2 * t + (k & 1) + 8 * (k >> 1)), 0);
+      float s[RT][4];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.f;
+      const uint8_t* kr[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        kr[k] = head_k + max(kslot[k], 0) / IMBA_PAGE_TOKENS * a.cache.page_stride +
+                max(kslot[k], 0) % IMBA_PAGE_TOKENS * DQK + t * D::VK;
+#pragma unroll
+      for (int c = 0; c < D::CK; ++c)
+#pragma unroll
+        for (int j = 0; j < D::VK / 4; ++j) {
+          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(kr[0] + c * 4 * D::VK + 4 * j);
+          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(kr[1] + c * 4 * D::VK + 4 * j);
+          const uint32_t ka[4] = {e4m3x2_to_h2(w0), e4m3x2_to_h2(w1), e4m3x2_to_h2(w0 >> 16), e4m3x2_to_h2(w1 >> 16)};
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+              mma_f16(s[r], ka, st.q[r][p][c * (D::VK / 4) + j][0], st.q[r][p][c * (D::VK / 4) + j][1]);
+        }
+      uint32_t pb[RT][NP][2];
+      st.weigh(s, ks, vb, kpos, a.call.max_pos, true,
+               [&](int r, int e, int k) { return kslot[k] >= 0 && kown[k] == 8 * r + 2 * t + e; }, pb);
+#pragma unroll
+      for (int c = 0; c < D::CV; ++c) {
+        // The two keys' codes of each dimension side by side.
+        uint32_t w[2][D::VV / 4];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t u[2][D::VV / 4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int sl = vslot[2 * k + e], tok = sl % IMBA_PAGE_TOKENS;
+            const uint8_t* v = head_k + v_from_k + sl / IMBA_PAGE_TOKENS * a.cache.page_stride +
+                               v8_off(tok & ~1, c * 4 * D::VV + g * (D::VV / 2), DV);
+#pragma unroll
+            for (int j = 0; j < D::VV / 4; ++j)
+              u[e][j] = *reinterpret_cast<const uint32_t*>(v + 4 * j) >> (8 * (tok & 1)) & 0x00ff00ffu;
+          }
+#pragma unroll
+          for (int j = 0; j < D::VV / 4; ++j) w[k][j] = u[0][j] | u[1][j] << 8;
+        }
+#pragma unroll
+        for (int j = 0; j < D::VV / 4; ++j) {
+          const uint32_t va[4] = {e4m3x2_to_h2(w[0][j]), e4m3x2_to_h2(w[0][j] >> 16), e4m3x2_to_h2(w[1][j]),
+                                  e4m3x2_to_h2(w[1][j] >> 16)};
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int p = 0; p < NP; ++p) mma_f16(st.o[r][c * (D::VV / 4) + j], va, pb[r][p][0], pb[r][p][1]);
+        }
+      }
+    }
   }
 
   // Out: true units, relative to each row's running maximum.
-  const float unit_v = vref ? scale_of(vref) : 1.f;
+  const float unit_v = st.vref ? scale_of(st.vref) : 1.f;
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int r = 0; r < 2; ++r) st.l[m][r] = quad_sum(st.l[m][r]);
+    for (int r = 0; r < 2; ++r) st.l[i][r] = keys_sum(st.l[i][r]);
   const bool ovec = a.call.out_stride[0] % 4 == 0 && a.call.out_stride[1] % 4 == 0 &&
                     (reinterpret_cast<uintptr_t>(a.call.out) & (4 * sizeof(T) - 1)) == 0;
+  // Dimensions e .. e + 3 of this lane's row i, r, times f; e = dim(c, q).
+  auto four = [&](int i, int r, int c, int q, float f, float (&x)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = st.o[i][c * (D::VV / 4) + (4 * q + j) / 2][2 * (j & 1) + r] * f;
+  };
+  auto dim = [&](int c, int q) { return c * 4 * D::VV + g * (D::VV / 2) + 4 * q; };
 
   if constexpr (NW == 1) {
     const size_t part = ((size_t)max(it.part, 0) * H + head) * D::ROWS;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const AttendRow& row = rows[m][r];
-        if (row.row < 0) continue;
-        const int tr = 16 * m + g + 8 * r;
-        const float f = it.part >= 0 ? unit_v : st.l[m][r] == 0.f ? 0.f : unit_v / st.l[m][r];
-        if (it.part >= 0 && t == 0) a.plan.ml[part + tr] = make_float2(st.m[m][r], st.l[m][r]);
-        T* out = static_cast<T*>(a.call.out) + row.row * a.call.out_stride[0] +
-                 (int64_t)(head * a.shape.share + row.head) * a.call.out_stride[1];
+        const int tr = 8 * i + 2 * t + r;
+        const int4 row = __ldg(tile + tr);
+        if (row.x < 0) continue;
+        const float f = it.part >= 0 ? unit_v : st.l[i][r] == 0.f ? 0.f : unit_v / st.l[i][r];
+        if (it.part >= 0 && g == 0) a.plan.ml[part + tr] = make_float2(st.m[i][r], st.l[i][r]);
+        T* out = static_cast<T*>(a.call.out) + row.x * a.call.out_stride[0] +
+                 (int64_t)(head * a.shape.share + row.w) * a.call.out_stride[1];
 #pragma unroll
         for (int c = 0; c < D::CV; ++c)
 #pragma unroll
-          for (int q = 0; q < D::VV / 4; ++q) {  // dimensions 4 VV c + VV t + 4 q .. + 3
+          for (int q = 0; q < D::VV / 8; ++q) {
             float x[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int d = 4 * q + j;
-              x[j] = o[m][c * (D::VV / 2) + d % (D::VV / 2)][2 * r + d / (D::VV / 2)] * f;
-            }
-            const int e = c * 4 * D::VV + t * D::VV + 4 * q;
+            four(i, r, c, q, f, x);
             if (it.part >= 0)
-              *reinterpret_cast<float4*>(a.plan.o + (part + tr) * DV + e) = make_float4(x[0], x[1], x[2], x[3]);
+              *reinterpret_cast<float4*>(a.plan.o + (part + tr) * DV + dim(c, q)) = make_float4(x[0], x[1], x[2], x[3]);
             else
-              out_store4(out + e, ovec, x);
+              out_store4(out + dim(c, q), ovec, x);
           }
       }
     if (it.part >= 0) {
@@ -575,7 +653,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, DQK <= 64 && MT == 1 && sizeo
       if (__shfl_sync(0xffffffffu, n, 0) == it.splits - 1) {  // the others have finished
         __threadfence();
         if (lane == 0) *done = 0;
-        join_items<T, DQK, DV, MT>(a, it, head, lane, 32);
+        join_items<T, DQK, DV, RT>(a, it, head, lane, 32);
       }
     }
   } else {
@@ -586,33 +664,28 @@ __global__ void __launch_bounds__(kUnitWarps * 32, DQK <= 64 && MT == 1 && sizeo
     cp_wait<0>();
     __syncthreads();
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int tr = 16 * m + g + 8 * r;
-        if (rows[m][r].row < 0) continue;
-        if (t == 0) sml[warp * D::ROWS + tr] = make_float2(st.m[m][r], st.l[m][r]);
+        const int tr = 8 * i + 2 * t + r;
+        if (__ldg(tile + tr).x < 0) continue;
+        if (g == 0) sml[warp * D::ROWS + tr] = make_float2(st.m[i][r], st.l[i][r]);
         float* dst = so + (warp * D::ROWS + tr) * DV;
 #pragma unroll
         for (int c = 0; c < D::CV; ++c)
 #pragma unroll
-          for (int q = 0; q < D::VV / 4; ++q) {
+          for (int q = 0; q < D::VV / 8; ++q) {
             float x[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int d = 4 * q + j;
-              x[j] = o[m][c * (D::VV / 2) + d % (D::VV / 2)][2 * r + d / (D::VV / 2)] * unit_v;
-            }
-            *reinterpret_cast<float4*>(dst + c * 4 * D::VV + t * D::VV + 4 * q) = make_float4(x[0], x[1], x[2], x[3]);
+            four(i, r, c, q, unit_v, x);
+            *reinterpret_cast<float4*>(dst + dim(c, q)) = make_float4(x[0], x[1], x[2], x[3]);
           }
       }
     __syncthreads();
     const size_t part = ((size_t)max(it.part, 0) * H + head) * D::ROWS;
     for (int i = threadIdx.x; i < D::ROWS * (DV / 4); i += kUnitWarps * 32) {
       const int tr = i / (DV / 4), e = i % (DV / 4) * 4;
-      const int4 u = __ldg(reinterpret_cast<const int4*>(tile + tr));
-      const AttendRow row{u.x, u.y, u.z, u.w};
-      if (row.row < 0) continue;
+      const int4 row = __ldg(tile + tr);
+      if (row.x < 0) continue;
       float mm = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kUnitWarps; ++w) mm = fmaxf(mm, sml[w * D::ROWS + tr].x);
@@ -631,8 +704,8 @@ __global__ void __launch_bounds__(kUnitWarps * 32, DQK <= 64 && MT == 1 && sizeo
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] *= inv;
-        out_store4(static_cast<T*>(a.call.out) + row.row * a.call.out_stride[0] +
-                       (int64_t)(head * a.shape.share + row.head) * a.call.out_stride[1] + e,
+        out_store4(static_cast<T*>(a.call.out) + row.x * a.call.out_stride[0] +
+                       (int64_t)(head * a.shape.share + row.w) * a.call.out_stride[1] + e,
                    ovec, x);
       }
     }
@@ -645,19 +718,21 @@ __global__ void __launch_bounds__(kUnitWarps * 32, DQK <= 64 && MT == 1 && sizeo
       if (*flag) {
         __threadfence();
         if (threadIdx.x == 0) *done = 0;
-        join_items<T, DQK, DV, MT>(a, it, head, threadIdx.x, kUnitWarps * 32);
+        join_items<T, DQK, DV, RT>(a, it, head, threadIdx.x, kUnitWarps * 32);
       }
     }
   }
 }
 
-template <typename T, int DQK, int DV, int MT, int NW>
+template <typename T, int DQK, int DV, int RT, int NW>
 cudaError_t launch_one(const AttendArgs& a, cudaStream_t s) {
-  using D = Dims<DQK, DV, MT>;
+  using D = Dims<DQK, DV, RT>;
   constexpr int kStages = 4;
+  // CTAs an SM by what a lane's rows take in registers
+  constexpr int kCtas = DQK > 64 ? (RT == 1 ? 2 : 1) : RT == 1 ? 3 : RT == 2 ? 2 : 1;
   constexpr size_t ring = (size_t)kUnitWarps * kStages * D::STAGE;
   constexpr size_t smem = NW > 1 && D::MERGE > ring ? D::MERGE : ring;
-  auto fn = attend8_kernel<T, DQK, DV, MT, NW, kStages>;
+  auto fn = attend8_kernel<T, DQK, DV, RT, NW, kStages, kCtas>;
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   const int64_t units = (int64_t)a.shape.max_items * a.cache.H;
@@ -666,14 +741,21 @@ cudaError_t launch_one(const AttendArgs& a, cudaStream_t s) {
   return launch_pdl(fn, dim3((unsigned)grid), dim3(kUnitWarps * 32), smem, s, a);
 }
 
+template <typename T, int DQK, int DV, int RT>
+cudaError_t launch_rows(const AttendArgs& a, cudaStream_t s) {
+  return a.shape.warps == 1 ? launch_one<T, DQK, DV, RT, 1>(a, s) : launch_one<T, DQK, DV, RT, kUnitWarps>(a, s);
+}
+
 }  // namespace
 
 template <typename T>
 cudaError_t launch_attend8(const imba_cache_desc& c, const AttendArgs& a, cudaStream_t s) {
-#define IMBA_ATTEND8(DQK, DV)                                                     \
-  if (c.attention_dim == DQK && c.linear_dim == DV)                               \
-    return a.shape.warps == 1 ? launch_one<T, DQK, DV, 1, 1>(a, s)                \
-                              : launch_one<T, DQK, DV, 1, kUnitWarps>(a, s);
+#define IMBA_ATTEND8(DQK, DV)                                              \
+  if (c.attention_dim == DQK && c.linear_dim == DV) {                      \
+    if (a.shape.rt == 1) return launch_rows<T, DQK, DV, 1>(a, s);          \
+    if (a.shape.rt == 2) return launch_rows<T, DQK, DV, 2>(a, s);          \
+    if constexpr (DV <= 64) return launch_rows<T, DQK, DV, 4>(a, s);       \
+  }
   IMBA_ATTEND8(32, 32)
   IMBA_ATTEND8(64, 64)
   IMBA_ATTEND8(32, 64)
