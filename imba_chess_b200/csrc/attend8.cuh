@@ -33,7 +33,7 @@ struct AttendItem {
 
 struct AttendShape {
   int share;        // query heads per key / value head
-  int rt;           // 8-row groups of a tile: 1, 2 or 4
+  int rt;           // 8-row groups of a tile: 1 or 2
   int warps;        // warps that share a unit: 1 or kUnitWarps
   int tile_rows;    // kTileRows * rt
   int max_tiles;

@@ -45,7 +45,6 @@ namespace {
 constexpr float kShift = 5.f;
 constexpr float kSlack = 4.f;
 constexpr int kVWindow = 6;  // 2^(kShift + kSlack + kVWindow) = 2^15 is finite in f16
-constexpr float kLowest = -3.402823466e38f;
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -117,14 +116,18 @@ __device__ __forceinline__ float keys_sum(float x) {
   return x;
 }
 
-// The bias in the log2 domain; a finite bias stays finite, so a row whose
-// every key carries the type's lowest value still weighs them alike.
-__device__ __forceinline__ float bias_log2(float b) {
-  return b == -INFINITY ? b : fmaxf(b * kLog2e, kLowest);
-}
+// Scores are kept in log2 without a bias (the factor log2 e joins the
+// query's), with one as natural logarithms, where the bias is added as it is;
+// `lg` takes them to log2.  A bias below kFar that is not -inf counts as
+// kFar, a power of two, whose product with lg is exact: a row whose every key
+// carries the type's lowest value still weighs its keys by nothing else.
+constexpr float kFar = -1.2676506002282294e30f;  // -2^100
+__device__ __forceinline__ float take_bias(float b) { return b == -INFINITY ? b : fmaxf(b, kFar); }
 
-// 2^(a - b) for running maxima; 0 for a part that has seen nothing.
-__device__ __forceinline__ float weight_of(float a, float b) { return a == -INFINITY ? 0.f : exp2_approx(a - b); }
+// exp of a difference of running maxima; 0 for a part that has seen nothing.
+__device__ __forceinline__ float weight_of(float a, float b, float lg) {
+  return a == -INFINITY ? 0.f : exp2_approx((a - b) * lg);
+}
 
 // Four consecutive elements of a row as floats.
 template <typename T>
@@ -173,7 +176,8 @@ struct Dims {
 
 // Tile rows joined over the items of a split tile; `nthr` threads from tid on.
 template <typename T, int DQK, int DV, int RT>
-__device__ __forceinline__ void join_items(const AttendArgs& a, const AttendItem& it, int head, int tid, int nthr) {
+__device__ __forceinline__ void join_items(const AttendArgs& a, const AttendItem& it, int head, float lg, int tid,
+                                           int nthr) {
   using D = Dims<DQK, DV, RT>;
   const int H = a.cache.H;
   const size_t first = (size_t)(it.part - it.index) * H + head;
@@ -190,7 +194,7 @@ __device__ __forceinline__ void join_items(const AttendArgs& a, const AttendItem
     for (int s = 0; s < it.splits; ++s) {
       const size_t at = (first + (size_t)s * H) * D::ROWS + r;
       const float2 ml = __ldcg(a.plan.ml + at);
-      const float w = weight_of(ml.x, m);
+      const float w = weight_of(ml.x, m, lg);
       const float4 o = __ldcg(reinterpret_cast<const float4*>(a.plan.o + at * DV + e));
       l += w * ml.y;
       x[0] += w * o.x, x[1] += w * o.y, x[2] += w * o.z, x[3] += w * o.w;
@@ -212,38 +216,25 @@ struct Rows {
   using D = Dims<DQK, DV, RT>;
   uint32_t q[RT][NP][D::KS][2];  // row 8 i + g: B fragments
   float fac[RT][2];              // of a raw score, without the block's scale
-  int vis[RT][2], pos[RT][2];
-  const float* bias[RT][2];      // the row's bias, or null
-  float m[RT][2], l[RT][2];      // running maximum (log2 domain), sum over this lane's keys
+  int vis[RT][2], pos[RT][2];    // visible tokens; the bias column of a key is its position plus pos, clamped
+  const float* bias[RT][2];      // the row's bias (the call has one, or none of them is read)
+  float m[RT][2], l[RT][2];      // running maximum, sum over this lane's keys
+  float ref[RT][2];              // kShift - lg m: a weight is 2^(lg score + ref)
+  float lg, slack;               // from scores to log2; kSlack in scores
   float o[RT][D::MV][4];
-  int vref;                      // scale byte that O is held in units of; 0: none yet
+  int vref, vmost;               // scale byte that O is held in units of, 0: none yet; the largest so far
 
-  bool uniform_scales;           // the sixteen keys share their scales (a page)
-
-  // Sixteen keys: from raw scores s (keys g and g + 8; their K scales, V
-  // scale bytes and positions) to weights, as B fragments in p.
-  template <class Mask>
-  __device__ __forceinline__ void weigh(float (&s)[RT][4], const float (&ks)[2], const int (&vb)[2],
-                                        const int (&kpos)[2], int max_pos, bool masked, const Mask& sees,
-                                        uint32_t (&p)[RT][NP][2]) {
+  // Sixteen keys' scores (keys g and g + 8; -inf: not seen) to weights times
+  // 2^up in place, summed up in l without it.
+  __device__ __forceinline__ void weigh(float (&s)[RT][4], float up, float down) {
     bool raise = false;
     float mx[RT][2];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        s[i][r] *= ks[0] * fac[i][r];
-        s[i][2 + r] *= ks[1] * fac[i][r];
-        if (bias[i][r]) {
-          s[i][r] += bias_log2(__ldg(bias[i][r] + bias_index(kpos[0], pos[i][r], max_pos)));
-          s[i][2 + r] += bias_log2(__ldg(bias[i][r] + bias_index(kpos[1], pos[i][r], max_pos)));
-        }
-        if (masked) {
-          if (!sees(i, r, 0)) s[i][r] = -INFINITY;
-          if (!sees(i, r, 1)) s[i][2 + r] = -INFINITY;
-        }
         mx[i][r] = fmaxf(s[i][r], s[i][2 + r]);
-        raise |= mx[i][r] > m[i][r] + kSlack;
+        raise |= mx[i][r] > m[i][r] + slack;
       }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -251,8 +242,9 @@ struct Rows {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float now = fmaxf(m[i][r], keys_max(mx[i][r]));
-          const float w = weight_of(m[i][r], now);
+          const float w = weight_of(m[i][r], now, lg);
           m[i][r] = now;
+          ref[i][r] = now == -INFINITY ? 0.f : fmaf(-now, lg, kShift);
           l[i][r] *= w;
 #pragma unroll
           for (int j = 0; j < D::MV; ++j) {
@@ -261,43 +253,40 @@ struct Rows {
           }
         }
     }
-    // V's scales as ratios to vref, which follows them.
-    float ratio[2] = {1.f, 1.f};
-    int top = max(vb[0], vb[1]), low = min(vb[0] ? vb[0] : 255, vb[1] ? vb[1] : 255);
-    if (!uniform_scales) {
-      top = __reduce_max_sync(0xffffffffu, top);
-      low = __reduce_min_sync(0xffffffffu, low);
-    }
-    if (top) {
-      if (vref == 0) vref = top;
-      if (top - vref > kVWindow || vref - low > kVWindow) {
-        const int now = max(top, vref - 60);
-        const float f = vref - now < -126 ? 0.f : __uint_as_float((uint32_t)(127 + vref - now) << 23);
-        vref = now;
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int j = 0; j < D::MV; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][j][e] *= f;
-      }
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-        if (vb[n]) ratio[n] = vb[n] - vref < -126 ? 0.f : __uint_as_float((uint32_t)(127 + vb[n] - vref) << 23);
-    }
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      float w[4];
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float ref = m[i][r] == -INFINITY ? 0.f : m[i][r] - kShift;
-        w[r] = exp2_approx(s[i][r] - ref);
-        w[2 + r] = exp2_approx(s[i][2 + r] - ref);
-        l[i][r] += w[r] + w[2 + r];
+        const float from = ref[i][r] + up;
+        s[i][r] = exp2_approx(fmaf(s[i][r], lg, from));
+        s[i][2 + r] = exp2_approx(fmaf(s[i][2 + r], lg, from));
+        l[i][r] = fmaf(s[i][r] + s[i][2 + r], down, l[i][r]);
       }
+  }
+
+  // Lets vref follow a block's V scale byte vb (not 0).  It stays within 2^80
+  // of the largest scale, so that no sum overflows in its units.
+  __device__ __forceinline__ void follow(int vb) {
+    if (vref == 0) vref = vb;
+    vmost = max(vmost, vb);
+    if (abs(vb - vref) <= kVWindow) return;
+    const int now = max(vb, vmost - 80);
+    const float f = vref - now < -126 ? 0.f : __uint_as_float((uint32_t)(127 + vref - now) << 23);
+    vref = now;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < D::MV; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][j][e] *= f;
+  }
+  // A block's weights as B fragments.
+  __device__ __forceinline__ void pack(const float (&w)[RT][4], uint32_t (&p)[RT][NP][2]) const {
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
       uint32_t lo[NP], hi[NP];
-      split_h2<NP>(w[0] * ratio[0], w[1] * ratio[0], lo);
-      split_h2<NP>(w[2] * ratio[1], w[3] * ratio[1], hi);
+      split_h2<NP>(w[i][0], w[i][1], lo);
+      split_h2<NP>(w[i][2], w[i][3], hi);
 #pragma unroll
       for (int n = 0; n < NP; ++n) {
         p[i][n][0] = transpose8(lo[n]);
@@ -317,17 +306,21 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int sub = NW == 1 ? 0 : warp;
   const int H = a.cache.H;
-  const int64_t unit = NW == 1 ? (int64_t)blockIdx.x * kUnitWarps + warp : blockIdx.x;
-  const int item_id = (int)(unit / H), head = (int)(unit % H);
-  if (item_id >= a.plan.head[0]) return;
-  const AttendItem it = a.plan.items[item_id];
+  const uint32_t unit = NW == 1 ? blockIdx.x * kUnitWarps + warp : blockIdx.x;
+  const int item_id = (int)(unit / (uint32_t)H), head = (int)(unit % (uint32_t)H);
+  if (item_id >= a.shape.max_items) return;
+  const int items = a.plan.head[0];
+  const AttendItem it = a.plan.items[item_id];  // together with the count
+  if (item_id >= items) return;
   const int4* tile = reinterpret_cast<const int4*>(a.plan.rows + (size_t)it.tile * D::ROWS);
 
   // This warp's pages: list entries sub, sub + NW, ... of the item, 32 at a
   // time in the lanes (id and the two scale bytes), the next 32 in flight.
   const int npages = it.pages > sub ? (it.pages - sub + NW - 1) / NW : 0;
   const uint8_t* head_k = a.cache.data + (int64_t)head * IMBA_PAGE_TOKENS * DQK;
+  const uint8_t* lane_k = head_k + g * DQK + t * D::VK;
   const int64_t v_from_k = a.cache.v_offset + (int64_t)head * IMBA_PAGE_TOKENS * (DV - DQK);
+  const uint8_t* lane_v = head_k + v_from_k + t * 2 * DV + g * D::VV;
   auto page_id = [&](int i) -> int {  // -1: none, -2: outside the pool
     if (i >= npages) return -1;
     const int id = a.rows.group_pages[it.list + sub + i * NW];
@@ -349,45 +342,42 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
     for (int r = 0; r < 2; ++r) {
       const int4 u = __ldg(tile + 8 * i + 2 * t + r);
       st.vis[i][r] = u.y;
-      st.pos[i][r] = u.z;
-      st.bias[i][r] = a.call.bias && u.x >= 0
-                          ? a.call.bias + (int64_t)(head * a.shape.share + u.w) * (2 * a.call.max_pos - 1)
-                          : nullptr;
+      st.pos[i][r] = a.call.max_pos - 1 - u.z;
+      st.bias[i][r] = a.call.bias + (int64_t)(head * a.shape.share + u.w) * (2 * a.call.max_pos - 1);
       st.m[i][r] = -INFINITY;
-      st.l[i][r] = 0.f;
+      st.l[i][r] = st.ref[i][r] = 0.f;
     }
 #pragma unroll
     for (int j = 0; j < D::MV; ++j) st.o[i][j][0] = st.o[i][j][1] = st.o[i][j][2] = st.o[i][j][3] = 0.f;
   }
-  st.vref = 0;
-  st.uniform_scales = true;
+  st.vref = st.vmost = 0;
+  st.lg = a.call.bias ? kLog2e : 1.f;
+  st.slack = a.call.bias ? kSlack / kLog2e : kSlack;
   int scs = page_scales(ids), scs_next = page_scales(ids_next);
   if (__any_sync(0xffffffffu, ids == -2 || ids_next == -2) && lane == 0) report(a.rows.status, IMBA_ERR_RANGE);
 
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (STAGES * D::STAGE);
-  auto issue = [&](int i, int batch) {  // page i of the warp into its stage; `batch` holds i's page id
+  auto issue = [&](int i, int batch, uint32_t dst) {  // page i of the warp; `batch` holds its id
     const int id = __shfl_sync(0xffffffffu, batch, i & 31);
     if (i < npages) {
-      const uint8_t* k = head_k + max(id, 0) * a.cache.page_stride;
-      const uint32_t dst = ring + i % STAGES * D::STAGE;
+      const uint8_t* k = lane_k + (uint64_t)(uint32_t)max(id, 0) * (uint32_t)a.cache.page_stride;
+      const uint8_t* v = lane_v + (uint64_t)(uint32_t)max(id, 0) * (uint32_t)a.cache.page_stride;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int c = 0; c < D::CK; ++c)
-          cp_async<D::VK>(dst + ((n * D::CK + c) * 32 + lane) * D::VK,
-                          k + (n * 8 + g) * DQK + c * 4 * D::VK + t * D::VK);
-      const uint8_t* v = k + v_from_k;
+          cp_async<D::VK>(dst + (n * D::CK + c) * 32 * D::VK + lane * D::VK, k + n * 8 * DQK + c * 4 * D::VK);
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int c = 0; c < D::CV; ++c)
-          cp_async<D::VV>(dst + IMBA_PAGE_TOKENS * DQK + ((n * D::CV + c) * 32 + lane) * D::VV,
-                          v + (n * 4 + t) * 2 * DV + c * 8 * D::VV + g * D::VV);
+          cp_async<D::VV>(dst + IMBA_PAGE_TOKENS * DQK + (n * D::CV + c) * 32 * D::VV + lane * D::VV,
+                          v + n * 8 * DV + c * 8 * D::VV);
     }
     cp_commit();
   };
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) issue(i, ids);
+  for (int i = 0; i < STAGES - 1; ++i) issue(i, ids, ring + i * D::STAGE);
 
   // Queries: f16 B fragments of each row over its power of two.
   const bool qvec = a.call.q_stride[0] % 4 == 0 && a.call.q_stride[1] % 4 == 0 &&
@@ -410,7 +400,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
     const int ex = (int)(__float_as_uint(amax) >> 23);  // 0 for a zero row, 255 for an infinite one
     const int e = ex == 0 || ex == 255 ? 0 : min(ex - 127, 126);
     const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-    const float f = __uint_as_float((uint32_t)(127 + e) << 23) * a.call.scale * kLog2e;
+    const float f = __uint_as_float((uint32_t)(127 + e) << 23) * (a.call.bias ? a.call.scale : a.call.scale * kLog2e);
     st.fac[i][0] = __shfl_sync(0xffffffffu, f, 8 * t);
     st.fac[i][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll
@@ -426,7 +416,22 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
     }
   }
 
-  for (int i = 0; i < npages; ++i) {
+  // Bias columns: within [0, last] nothing is clamped.
+  const bool biased = a.call.bias != nullptr;
+  const int last = 2 * a.call.max_pos - 2;
+  bool inside = true;
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      inside &= it.key0 + st.pos[r][e] >= 0 && it.key0 + it.pages * IMBA_PAGE_TOKENS + st.pos[r][e] <= last + 1;
+      if (biased) st.bias[r][e] += g;
+    }
+  inside = __all_sync(0xffffffffu, inside);
+
+  uint32_t from = ring, into = ring + (STAGES - 1) * D::STAGE;
+  int key0 = it.key0 + sub * IMBA_PAGE_TOKENS;
+  for (int i = 0; i < npages; ++i, key0 += NW * IMBA_PAGE_TOKENS) {
     if (i && (i & 31) == 0) {
       ids = ids_next;
       scs = scs_next;
@@ -435,28 +440,43 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
       if (__any_sync(0xffffffffu, ids_next == -2) && lane == 0) report(a.rows.status, IMBA_ERR_RANGE);
     }
     const int sc = __shfl_sync(0xffffffffu, scs, i & 31);
-    const int id = __shfl_sync(0xffffffffu, ids, i & 31);
-    {
-      const int ahead = i + STAGES - 1;
-      const int batch = (ahead >> 5) == (i >> 5) ? ids : ids_next;
-      cp_wait<STAGES - 2>();  // page i has arrived
-      issue(ahead, batch);    // into the stage that page i - 1 left
+    float s[RT][4], add[RT][4];
+    if (biased) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (inside) {
+            const float* at = st.bias[r][e] + (key0 + st.pos[r][e]);
+            add[r][e] = __ldg(at);
+            add[r][2 + e] = __ldg(at + 8);
+          } else {
+            const float* at = st.bias[r][e] - g;
+            const int col = key0 + g + st.pos[r][e];
+            add[r][e] = __ldg(at + min(max(col, 0), last));
+            add[r][2 + e] = __ldg(at + min(max(col + 8, 0), last));
+          }
+        }
     }
-    const uint32_t src = ring + i % STAGES * D::STAGE;
-    const int key0 = it.key0 + (sub + i * NW) * IMBA_PAGE_TOKENS;
+    cp_wait<STAGES - 2>();  // page i has arrived
+    {
+      const int ahead = i + STAGES - 1;  // into the stage that page i - 1 left
+      issue(ahead, (ahead ^ i) & 32 ? ids_next : ids, into);
+      into = into + D::STAGE == ring + STAGES * D::STAGE ? ring : into + D::STAGE;
+    }
 
-    float s[RT][4];
 #pragma unroll
     for (int r = 0; r < RT; ++r) s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.f;
 #pragma unroll
     for (int c = 0; c < D::CK; ++c) {
       uint32_t w0[D::VK / 4], w1[D::VK / 4];
-      lds<D::VK>(src + (c * 32 + lane) * D::VK, w0);
-      lds<D::VK>(src + ((D::CK + c) * 32 + lane) * D::VK, w1);
+      lds<D::VK>(from + c * 32 * D::VK + lane * D::VK, w0);
+      lds<D::VK>(from + (D::CK + c) * 32 * D::VK + lane * D::VK, w1);
 #pragma unroll
       for (int j = 0; j < D::VK / 4; ++j) {
-        const uint32_t ka[4] = {e4m3x2_to_h2(w0[j]), e4m3x2_to_h2(w1[j]), e4m3x2_to_h2(w0[j] >> 16),
-                                e4m3x2_to_h2(w1[j] >> 16)};
+        uint32_t ka[4];
+        e4m3x4_to_h2(w0[j], ka[0], ka[2]);
+        e4m3x4_to_h2(w1[j], ka[1], ka[3]);
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -464,27 +484,60 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
             mma_f16(s[r], ka, st.q[r][p][c * (D::VK / 4) + j][0], st.q[r][p][c * (D::VK / 4) + j][1]);
       }
     }
-
-    const float ks[2] = {scale_of(sc & 255), scale_of(sc & 255)};
-    const int vb[2] = {sc >> 8, sc >> 8}, kpos[2] = {key0 + g, key0 + g + 8};
+    const float ks = scale_of(sc & 255);
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float f = ks * st.fac[r][e];
+        s[r][e] *= f;
+        s[r][2 + e] *= f;
+      }
+    if (biased) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[r][e] += take_bias(add[r][e]);
+    }
+    const int id = __shfl_sync(0xffffffffu, ids, i & 31);
+    if (key0 + IMBA_PAGE_TOKENS > it.minvis || id < 0) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int lim = id < 0 ? 0 : st.vis[r][e] - key0 - g;
+          if (lim <= 0) s[r][e] = -INFINITY;
+          if (lim <= 8) s[r][2 + e] = -INFINITY;
+        }
+    }
+    // V's scale as its ratio to vref, in the weights' exponent.
+    const int vb = sc >> 8;
+    if ((uint32_t)(vb - st.vref + kVWindow) > 2 * kVWindow && vb) st.follow(vb);
+    const int up = vb ? max(vb - st.vref, -126) : 0;
+    st.weigh(s, (float)up, __uint_as_float((uint32_t)(127 - up) << 23));
     uint32_t pb[RT][NP][2];
-    st.weigh(s, ks, vb, kpos, a.call.max_pos, id < 0 || key0 + IMBA_PAGE_TOKENS > it.minvis,
-             [&](int r, int e, int n) { return id >= 0 && kpos[n] < st.vis[r][e]; }, pb);
+    st.pack(s, pb);
 #pragma unroll
     for (int c = 0; c < D::CV; ++c) {
       uint32_t w0[D::VV / 4], w1[D::VV / 4];
-      lds<D::VV>(src + IMBA_PAGE_TOKENS * DQK + (c * 32 + lane) * D::VV, w0);
-      lds<D::VV>(src + IMBA_PAGE_TOKENS * DQK + ((D::CV + c) * 32 + lane) * D::VV, w1);
+      lds<D::VV>(from + IMBA_PAGE_TOKENS * DQK + c * 32 * D::VV + lane * D::VV, w0);
+      lds<D::VV>(from + IMBA_PAGE_TOKENS * DQK + (D::CV + c) * 32 * D::VV + lane * D::VV, w1);
 #pragma unroll
       for (int j = 0; j < D::VV / 4; ++j) {
-        const uint32_t va[4] = {e4m3x2_to_h2(w0[j]), e4m3x2_to_h2(w0[j] >> 16), e4m3x2_to_h2(w1[j]),
-                                e4m3x2_to_h2(w1[j] >> 16)};
+        uint32_t va[4];
+        e4m3x4_to_h2(w0[j], va[0], va[1]);
+        e4m3x4_to_h2(w1[j], va[2], va[3]);
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
           for (int p = 0; p < NP; ++p) mma_f16(st.o[r][c * (D::VV / 4) + j], va, pb[r][p][0], pb[r][p][1]);
       }
     }
+    from = from + D::STAGE == ring + STAGES * D::STAGE ? ring : from + D::STAGE;
+  }
+  if (biased) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) st.bias[r][0] -= g, st.bias[r][1] -= g;
   }
 
   // The rows' extra keys, sixteen of the tile's at a time: each is seen by
@@ -510,7 +563,6 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
       if (lane >= o) upto += y;
     }
     const int total = __shfl_sync(0xffffffffu, upto, 31);
-    st.uniform_scales = false;
     for (int x0 = 0; x0 < total; x0 += 16) {
       // Lane x holds key x0 + x: its row, slot, position and scales.
       int owner = 0, slot = -1, kp = 0, sc = 0;
@@ -562,45 +614,77 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
         for (int j = 0; j < D::VK / 4; ++j) {
           const uint32_t w0 = *reinterpret_cast<const uint32_t*>(kr[0] + c * 4 * D::VK + 4 * j);
           const uint32_t w1 = *reinterpret_cast<const uint32_t*>(kr[1] + c * 4 * D::VK + 4 * j);
-          const uint32_t ka[4] = {e4m3x2_to_h2(w0), e4m3x2_to_h2(w1), e4m3x2_to_h2(w0 >> 16), e4m3x2_to_h2(w1 >> 16)};
+          uint32_t ka[4];
+          e4m3x4_to_h2(w0, ka[0], ka[2]);
+          e4m3x4_to_h2(w1, ka[1], ka[3]);
 #pragma unroll
           for (int r = 0; r < RT; ++r)
 #pragma unroll
             for (int p = 0; p < NP; ++p)
               mma_f16(s[r], ka, st.q[r][p][c * (D::VK / 4) + j][0], st.q[r][p][c * (D::VK / 4) + j][1]);
         }
-      uint32_t pb[RT][NP][2];
-      st.weigh(s, ks, vb, kpos, a.call.max_pos, true,
-               [&](int r, int e, int k) { return kslot[k] >= 0 && kown[k] == 8 * r + 2 * t + e; }, pb);
 #pragma unroll
-      for (int c = 0; c < D::CV; ++c) {
-        // The two keys' codes of each dimension side by side.
-        uint32_t w[2][D::VV / 4];
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = e >> 1;
+          s[r][e] *= ks[k] * st.fac[r][e & 1];
+          if (biased)
+            s[r][e] += take_bias(__ldg(st.bias[r][e & 1] + min(max(kpos[k] + st.pos[r][e & 1], 0), last)));
+          if (kslot[k] < 0 || kown[k] != 8 * r + 2 * t + (e & 1)) s[r][e] = -INFINITY;
+        }
+      st.weigh(s, 0.f, 1.f);
+      // Keys whose V scales are too far apart for one reference take turns.
+      bool left[2] = {vb[0] > 0, vb[1] > 0};
+      do {
+        const int top = __reduce_max_sync(0xffffffffu, max(left[0] ? vb[0] : 0, left[1] ? vb[1] : 0));
+        if (top == 0) break;
+        st.follow(top);
+        float w[RT][4];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          uint32_t u[2][D::VV / 4];
+          const bool now = left[k] && vb[k] > top - kVWindow;
+          const float f = now ? __uint_as_float((uint32_t)max(127 + vb[k] - st.vref, 0) << 23) : 0.f;
+          left[k] = left[k] && !now;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int sl = vslot[2 * k + e], tok = sl % IMBA_PAGE_TOKENS;
-            const uint8_t* v = head_k + v_from_k + sl / IMBA_PAGE_TOKENS * a.cache.page_stride +
-                               v8_off(tok & ~1, c * 4 * D::VV + g * (D::VV / 2), DV);
+          for (int r = 0; r < RT; ++r) {
+            w[r][2 * k] = s[r][2 * k] * f;
+            w[r][2 * k + 1] = s[r][2 * k + 1] * f;
+          }
+        }
+        uint32_t pb[RT][NP][2];
+        st.pack(w, pb);
 #pragma unroll
-            for (int j = 0; j < D::VV / 4; ++j)
-              u[e][j] = *reinterpret_cast<const uint32_t*>(v + 4 * j) >> (8 * (tok & 1)) & 0x00ff00ffu;
+        for (int c = 0; c < D::CV; ++c) {
+          // The two keys' codes of each dimension side by side.
+          uint32_t w[2][D::VV / 4];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            uint32_t u[2][D::VV / 4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int sl = vslot[2 * k + e], tok = sl % IMBA_PAGE_TOKENS;
+              const uint8_t* v = head_k + v_from_k + sl / IMBA_PAGE_TOKENS * a.cache.page_stride +
+                                 v8_off(tok & ~1, c * 4 * D::VV + g * (D::VV / 2), DV);
+#pragma unroll
+              for (int j = 0; j < D::VV / 4; ++j)
+                u[e][j] = *reinterpret_cast<const uint32_t*>(v + 4 * j) >> (8 * (tok & 1)) & 0x00ff00ffu;
+            }
+#pragma unroll
+            for (int j = 0; j < D::VV / 4; ++j) w[k][j] = u[0][j] | u[1][j] << 8;
           }
 #pragma unroll
-          for (int j = 0; j < D::VV / 4; ++j) w[k][j] = u[0][j] | u[1][j] << 8;
+          for (int j = 0; j < D::VV / 4; ++j) {
+            uint32_t va[4];
+            e4m3x4_to_h2(w[0][j], va[0], va[1]);
+            e4m3x4_to_h2(w[1][j], va[2], va[3]);
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+              for (int p = 0; p < NP; ++p) mma_f16(st.o[r][c * (D::VV / 4) + j], va, pb[r][p][0], pb[r][p][1]);
+          }
         }
-#pragma unroll
-        for (int j = 0; j < D::VV / 4; ++j) {
-          const uint32_t va[4] = {e4m3x2_to_h2(w[0][j]), e4m3x2_to_h2(w[0][j] >> 16), e4m3x2_to_h2(w[1][j]),
-                                  e4m3x2_to_h2(w[1][j] >> 16)};
-#pragma unroll
-          for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int p = 0; p < NP; ++p) mma_f16(st.o[r][c * (D::VV / 4) + j], va, pb[r][p][0], pb[r][p][1]);
-        }
-      }
+      } while (true);
     }
   }
 
@@ -653,7 +737,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
       if (__shfl_sync(0xffffffffu, n, 0) == it.splits - 1) {  // the others have finished
         __threadfence();
         if (lane == 0) *done = 0;
-        join_items<T, DQK, DV, RT>(a, it, head, lane, 32);
+        join_items<T, DQK, DV, RT>(a, it, head, st.lg, lane, 32);
       }
     }
   } else {
@@ -692,7 +776,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
 #pragma unroll
       for (int w = 0; w < kUnitWarps; ++w) {
         const float2 ml = sml[w * D::ROWS + tr];
-        const float f = weight_of(ml.x, mm);
+        const float f = weight_of(ml.x, mm, st.lg);
         const float4 v = *reinterpret_cast<const float4*>(so + (w * D::ROWS + tr) * DV + e);
         l += f * ml.y;
         x[0] += f * v.x, x[1] += f * v.y, x[2] += f * v.z, x[3] += f * v.w;
@@ -718,7 +802,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
       if (*flag) {
         __threadfence();
         if (threadIdx.x == 0) *done = 0;
-        join_items<T, DQK, DV, RT>(a, it, head, threadIdx.x, kUnitWarps * 32);
+        join_items<T, DQK, DV, RT>(a, it, head, st.lg, threadIdx.x, kUnitWarps * 32);
       }
     }
   }
@@ -727,9 +811,9 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
 template <typename T, int DQK, int DV, int RT, int NW>
 cudaError_t launch_one(const AttendArgs& a, cudaStream_t s) {
   using D = Dims<DQK, DV, RT>;
-  constexpr int kStages = 4;
+  constexpr int kStages = 3;
   // CTAs an SM by what a lane's rows take in registers
-  constexpr int kCtas = DQK > 64 ? (RT == 1 ? 2 : 1) : RT == 1 ? 3 : RT == 2 ? 2 : 1;
+  constexpr int kCtas = DQK > 64 ? (RT == 1 ? 2 : 1) : RT == 1 ? 3 : 2;
   constexpr size_t ring = (size_t)kUnitWarps * kStages * D::STAGE;
   constexpr size_t smem = NW > 1 && D::MERGE > ring ? D::MERGE : ring;
   auto fn = attend8_kernel<T, DQK, DV, RT, NW, kStages, kCtas>;
@@ -737,7 +821,7 @@ cudaError_t launch_one(const AttendArgs& a, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   const int64_t units = (int64_t)a.shape.max_items * a.cache.H;
   const int64_t grid = NW == 1 ? (units + kUnitWarps - 1) / kUnitWarps : units;
-  if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  if (units > INT32_MAX) return cudaErrorInvalidValue;
   return launch_pdl(fn, dim3((unsigned)grid), dim3(kUnitWarps * 32), smem, s, a);
 }
 
@@ -753,8 +837,7 @@ cudaError_t launch_attend8(const imba_cache_desc& c, const AttendArgs& a, cudaSt
 #define IMBA_ATTEND8(DQK, DV)                                              \
   if (c.attention_dim == DQK && c.linear_dim == DV) {                      \
     if (a.shape.rt == 1) return launch_rows<T, DQK, DV, 1>(a, s);          \
-    if (a.shape.rt == 2) return launch_rows<T, DQK, DV, 2>(a, s);          \
-    if constexpr (DV <= 64) return launch_rows<T, DQK, DV, 4>(a, s);       \
+    return launch_rows<T, DQK, DV, 2>(a, s);                               \
   }
   IMBA_ATTEND8(32, 32)
   IMBA_ATTEND8(64, 64)

@@ -200,7 +200,7 @@ AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r) {
   const int64_t flat = (int64_t)r.num_rows * sh.share;
   // Rows of a tile by what a segment has on average.
   const int64_t per_seg = r.num_segs ? (flat + r.num_segs - 1) / r.num_segs : 0;
-  sh.rt = per_seg <= 8 ? 1 : per_seg <= 16 || c.linear_dim > 64 ? 2 : 4;
+  sh.rt = per_seg <= 8 ? 1 : 2;
   sh.tile_rows = kTileRows * sh.rt;
   const int64_t tiles = r.num_segs ? (flat + sh.tile_rows - 1) / sh.tile_rows + r.num_segs : 0;
   sh.max_tiles = (int)std::min<int64_t>(tiles, INT32_MAX);

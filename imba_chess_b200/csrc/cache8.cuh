@@ -84,6 +84,12 @@ __device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t two) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
   return r;
 }
+// Four codes: the first two, and the last two.
+__device__ __forceinline__ void e4m3x4_to_h2(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
+}
 __device__ __forceinline__ float2 e4m3x2_to_f2(uint32_t two) {
   const uint32_t h = e4m3x2_to_h2(two);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));

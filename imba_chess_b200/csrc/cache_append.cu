@@ -861,7 +861,10 @@ imba_status_t validate_cache(const imba_cache_desc* c) {
   if (c->dtype < IMBA_DTYPE_F32 || c->dtype > IMBA_DTYPE_E4M3) return IMBA_ERR_ARG;
   if (c->attention_dim > 128 || c->linear_dim > 128 || c->num_heads > 1024 || c->num_layers > 1024)
     return IMBA_ERR_UNSUPPORTED;
-  if (c->dtype == IMBA_DTYPE_E4M3 && !cache8_dims_ok(c->attention_dim, c->linear_dim)) return IMBA_ERR_UNSUPPORTED;
+  // (a page's bytes in 8 bits are a 32-bit factor of the kernels' addresses)
+  if (c->dtype == IMBA_DTYPE_E4M3 &&
+      (!cache8_dims_ok(c->attention_dim, c->linear_dim) || cache8_page_bytes(*c) > UINT32_MAX))
+    return IMBA_ERR_UNSUPPORTED;
   return IMBA_OK;
 }
 
