@@ -42,9 +42,17 @@ struct AppendArgs {
   imba_rotary_desc rot;
   const int32_t* slots;
   int32_t* status;
-  int q_blocks;  // CTAs that turn queries (the first ones), a warp a row
+  int page_blocks;  // CTAs that store (the first ones); the others turn queries
+  int q_rows;       // rows of a query warp
   int64_t num_slots;
 };
+
+// The largest magnitude; a NaN stays one.
+__device__ __forceinline__ float most3(float m, float x, float y) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(x), "f"(y));
+  return r;
+}
 
 // Eight elements of the source type as they are in memory.
 template <typename T>
@@ -67,11 +75,11 @@ struct Raw8<bf16> {
       x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
-  // Largest magnitude as a float's bits, together with `most`.
-  __device__ __forceinline__ uint32_t see(uint32_t most) const {
+  // The largest magnitude, together with `most` (a NaN stays one).
+  __device__ __forceinline__ float see(float most) const {
     const uint32_t a = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu),
                                 __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
-    return max(most, max(a << 16, a & 0xffff0000u));
+    return most3(most, __uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
   }
 };
 template <>
@@ -87,12 +95,9 @@ struct Raw8<float> {
     x[0] = f[0].x, x[1] = f[0].y, x[2] = f[0].z, x[3] = f[0].w;
     x[4] = f[1].x, x[5] = f[1].y, x[6] = f[1].z, x[7] = f[1].w;
   }
-  __device__ __forceinline__ uint32_t see(uint32_t most) const {
-    float x[8];
-    get(x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
-    return most;
+  __device__ __forceinline__ float see(float most) const {
+    most = most3(most3(most, f[0].x, f[0].y), f[0].z, f[0].w);
+    return most3(most3(most, f[1].x, f[1].y), f[1].z, f[1].w);
   }
 };
 
@@ -155,11 +160,16 @@ struct Pairs {
   }
   // The elements turned by cs[p0 ..], in the order of memory of a and b.
   __device__ __forceinline__ void turned(const float2* cs, const PairMap& m, int p0, float (&x)[8], float (&y)[8]) const {
+    turned_by(reinterpret_cast<const float4*>(cs + p0), cs, m, p0, x, y);
+  }
+  // t: the eight pairs' turns, two each (fast).
+  template <class Four>
+  __device__ __forceinline__ void turned_by(const Four& t, const float2* cs, const PairMap& m, int p0, float (&x)[8],
+                                            float (&y)[8]) const {
     a.get(x);
     b.get(y);
     if constexpr (Fast) {
       if (p0 >= m.half) return;  // eight pairs turn, or none does
-      const float4* t = reinterpret_cast<const float4*>(cs + p0);
       if (m.inter) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -256,35 +266,55 @@ struct RowLanes {
   static constexpr int kHeads = 32 / kLanes;
 };
 
-// A warp turns one row of `heads` heads from src to dst (head strides sh, dh).
-template <typename T, typename TO, int D, bool Fast>
-__device__ __forceinline__ void turn_row(const imba_rotary_desc& rot, int64_t r, int heads, const T* src,
-                                         const Strides& ss, TO* dst, const Strides& ds, float2* cs) {
+// A warp turns rows r0 .. r0 + n - 1 (n <= N; those in the mask `live`) of
+// `heads` heads, from src to dst(row).  N rows' turns go to cs[0 .. N - 1].
+template <int N, typename T, typename TO, int D, bool Fast, class Dst>
+__device__ __forceinline__ void turn_rows(const imba_rotary_desc& rot, int64_t r0, uint32_t live, int heads,
+                                          const T* src, const Strides& ss, const Dst& dst, const Strides& ds,
+                                          float2 (*cs)[kMaxPairs]) {
   using L = RowLanes<D / 16>;
-  constexpr int kAhead = sizeof(T) == 2 ? 4 : 2;
+  constexpr int kAhead = sizeof(T) == 2 ? 4 : 2;  // passes in flight; a pass is kHeads heads of a row
   const int lane = threadIdx.x % 32, l = lane % L::kLanes, p0 = l * 8;
   const PairMap m{rot.rot_dim / 2, rot.interleaved};
+  const int groups = (heads + L::kHeads - 1) / L::kHeads, passes = groups * (N == 1 ? 1 : 32 - __clz(live));
   bool filled = false;
-  for (int h0 = 0; h0 < heads; h0 += kAhead * L::kHeads) {
+  float4 mine[4];  // the turns of this lane's pairs, of a single row (fast)
+  for (int j0 = 0; j0 < passes; j0 += kAhead) {
     Pairs<T, Fast> raw[kAhead];
+    auto place = [&](int i, int* row, int* h) {
+      const int j = j0 + i;
+      *row = N == 1 ? 0 : j / groups;
+      *h = (j - *row * groups) * L::kHeads + lane / L::kLanes;
+      return j < passes && live >> *row & 1 && *h < heads && l < D / 16;
+    };
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int h = h0 + i * L::kHeads + lane / L::kLanes;
-      if (h < heads && l < D / 16) raw[i].load(src + h * ss.head, ss, m, p0);
+      int row, h;
+      if (place(i, &row, &h)) raw[i].load(src + (r0 + row) * ss.row + h * ss.head, ss, m, p0);
     }
     if (!filled) {  // behind the first loads
-      __syncwarp();  // the last row's are done with
-      for (int p = lane; p < m.half; p += 32) cs[p] = row_turn(rot, r, p);
+      __syncwarp();  // the last rows' are done with
+#pragma unroll
+      for (int row = 0; row < N; ++row)
+        if (live >> row & 1)
+          for (int p = lane; p < m.half; p += 32) cs[row][p] = row_turn(rot, r0 + row, p);
       __syncwarp();
+      if constexpr (N == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine[i] = reinterpret_cast<const float4*>(cs[0] + min(p0, D / 2 - 8))[i];
+      }
       filled = true;
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int h = h0 + i * L::kHeads + lane / L::kLanes;
-      if (h >= heads || l >= D / 16) continue;
+      int row, h;
+      if (!place(i, &row, &h)) continue;
       float x[8], y[8];
-      raw[i].turned(cs, m, p0, x, y);
-      Pairs<T, Fast>::store(dst + h * ds.head, ds, m, p0, x, y);
+      if constexpr (N == 1)
+        raw[i].turned_by(mine, cs[0], m, p0, x, y);
+      else
+        raw[i].turned(cs[row], m, p0, x, y);
+      Pairs<T, Fast>::store(dst(r0 + row) + h * ds.head, ds, m, p0, x, y);
     }
   }
 }
@@ -312,18 +342,33 @@ __device__ __forceinline__ void turn_row_any(const imba_rotary_desc& rot, int64_
   }
 }
 
-// The row of a query warp; -1: past the end, padding or outside the pool.
-__device__ __forceinline__ int64_t query_row(const AppendArgs& a) {
-  const int64_t r = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
-  if (r >= a.n) return -1;
-  const int64_t slot = a.slots[r];
-  return slot >= 0 && slot < a.num_slots ? r : -1;
+// The first row of a query warp, and which of its rows have a slot in the pool.
+__device__ __forceinline__ int64_t query_rows(const AppendArgs& a, uint32_t* live) {
+  const int64_t r0 = ((int64_t)(blockIdx.x - a.page_blocks) * kWarps + threadIdx.x / 32) * a.q_rows;
+  const int64_t r = r0 + threadIdx.x % 32;
+  const int64_t slot = threadIdx.x % 32 < a.q_rows && r < a.n ? a.slots[r] : -1;
+  *live = __ballot_sync(0xffffffffu, slot >= 0 && slot < a.num_slots);
+  return r0;
 }
 
-// Largest magnitude as bits (a NaN's are above infinity's).
-__device__ __forceinline__ uint32_t see(const float (&x)[8], uint32_t most) {
+// The queries of a warp: a row, or with many of them kQueryRows, so that the
+// loads of several are in flight at once.
+constexpr int kQueryRows = 2 * kTok / kWarps;
+template <typename T, int D, bool Fast>
+__device__ __forceinline__ void turn_queries(const AppendArgs& a, float2 (*cs)[kMaxPairs]) {
+  uint32_t live;
+  const int64_t r0 = query_rows(a, &live);
+  if (!live) return;
+  auto dst = [&](int64_t r) { return static_cast<T*>(a.q_out) + r * a.qo.row; };
+  if (a.q_rows == 1)
+    turn_rows<1, T, T, D, Fast>(a.rot, r0, live, a.Hq, static_cast<const T*>(a.q), a.qs, dst, a.qo, cs);
+  else
+    turn_rows<kQueryRows, T, T, D, Fast>(a.rot, r0, live, a.Hq, static_cast<const T*>(a.q), a.qs, dst, a.qo, cs);
+}
+
+__device__ __forceinline__ float see(const float (&x)[8], float most) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+  for (int i = 0; i < 8; i += 2) most = most3(most, x[i], x[i + 1]);
   return most;
 }
 // What is not finite becomes zero, and the last half step below 2^128 does
@@ -358,8 +403,8 @@ __device__ __forceinline__ void rescale16(uint4* p, float f) {
 
 // The block's new scale byte, its earlier codes rounded to it (whole warp).
 template <int D>
-__device__ __forceinline__ int grow_scale(uint8_t* block, uint8_t* scale, int was, uint32_t most, int lane) {
-  const int now = max(was, scale_byte(__uint_as_float(__reduce_max_sync(0xffffffffu, most))));
+__device__ __forceinline__ int grow_scale(uint8_t* block, uint8_t* scale, int was, float most, int lane) {
+  const int now = max(was, scale_byte(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)))));
   if (now > was) {
     if (was > 0) {
       const float f = shrink(was, now);
@@ -425,7 +470,7 @@ struct KBlock {
                                       uint8_t* scale, bool& bad) const {
     const PairMap m{a.rot.rot_dim / 2, a.rot.interleaved};
     const int lane = threadIdx.x % 32, p0 = lane % kLanes * 8;
-    uint32_t most = 0;
+    float most = 0.f;
 #pragma unroll
     for (int i = 0; i < kPass; ++i) {
       const int t = token(i);
@@ -434,9 +479,9 @@ struct KBlock {
       raw[i].turned(cs[t], m, p0, x, y);
       most = see(x, see(y, most));
     }
-    const bool odd = __any_sync(0xffffffffu, most > __float_as_uint(kLargest));
+    const bool odd = __any_sync(0xffffffffu, !(most <= kLargest));
     if (odd) {
-      most = 0;
+      most = 0.f;
 #pragma unroll
       for (int i = 0; i < kPass; ++i) {
         const int t = token(i);
@@ -495,12 +540,12 @@ struct VBlock {
   __device__ __forceinline__ void put(const AppendArgs& a, const int* rows, uint8_t* block, uint8_t* scale,
                                       bool& bad) const {
     const int lane = threadIdx.x % 32, e = lane % kLanes * 8;
-    uint32_t most = 0;
+    float most = 0.f;
 #pragma unroll
     for (int i = 0; i < kPass; ++i) most = raw[i][0].see(raw[i][1].see(most));
-    const bool odd = __any_sync(0xffffffffu, most > __float_as_uint(kLargest));
+    const bool odd = __any_sync(0xffffffffu, !(most <= kLargest));
     if (odd) {
-      most = 0;
+      most = 0.f;
 #pragma unroll
       for (int i = 0; i < kPass; ++i)
 #pragma unroll
@@ -548,10 +593,10 @@ struct VBlock {
 // The single new token of a page, offset t, in one head of K or V: the
 // codes' scale (kLanes lanes a head; every lane of the warp takes part).
 template <int D, int kLanes, int kUsed>
-__device__ __forceinline__ int one_scale(uint8_t* block, uint8_t* scale, int was, uint32_t most, bool live, bool* again) {
+__device__ __forceinline__ int one_scale(uint8_t* block, uint8_t* scale, int was, float most, bool live, bool* again) {
 #pragma unroll
-  for (int o = 1; o < kLanes; o *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-  const int l = threadIdx.x % kLanes, now = max(was, scale_byte(__uint_as_float(most)));
+  for (int o = 1; o < kLanes; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const int l = threadIdx.x % kLanes, now = max(was, scale_byte(most));
   *again = live && now > was && was > 0;
   if (*again)
     for (int i = l; i < D * kTok / 16; i += kUsed) rescale16(reinterpret_cast<uint4*>(block) + i, shrink(was, now));
@@ -587,11 +632,11 @@ __device__ __forceinline__ void one_k8(const AppendArgs& a, int64_t r, int t, ui
     }
     float x[8], y[8];
     raw.turned(cs, m, min(p0, D / 2 - 8), x, y);
-    uint32_t most = see(x, see(y, 0));
-    if (most > __float_as_uint(kLargest)) {
+    float most = see(x, see(y, 0.f));
+    if (!(most <= kLargest)) {
       take_finite(x, bad);
       take_finite(y, bad);
-      most = see(x, see(y, 0));
+      most = see(x, see(y, 0.f));
     }
     __syncwarp();
     bool again;
@@ -629,10 +674,10 @@ __device__ __forceinline__ void one_v8(const AppendArgs& a, int64_t r, int t, ui
       uint8_t* block = blocks + (int64_t)h * kTok * D;
       float x[8];
       raw[i].get(x);
-      uint32_t most = raw[i].see(0);
-      if (most > __float_as_uint(kLargest)) {
+      float most = raw[i].see(0.f);
+      if (!(most <= kLargest)) {
         take_finite(x, bad);
-        most = see(x, 0);
+        most = see(x, 0.f);
       }
       __syncwarp();
       bool again;
@@ -662,63 +707,84 @@ constexpr int append_ctas(int bytes, int d) { return bytes * d <= 128 ? 3 : byte
 template <typename T, int DQK, int DV, bool Fast>
 __global__ void __launch_bounds__(kThreads, append_ctas(sizeof(T), DQK > DV ? DQK : DV))
     append8_kernel(AppendArgs a, Cache8 c) {
-  __shared__ int rows[2][kTok];
-  __shared__ __align__(16) float2 cs[kTok][kMaxPairs];
+  __shared__ int rows[3][kTok];
+  __shared__ __align__(16) float2 cs[2][kTok][kMaxPairs];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if ((int)blockIdx.x < a.q_blocks) {
-    const int64_t r = query_row(a);
-    if (r >= 0)
-      turn_row<T, T, DQK, Fast>(a.rot, r, a.Hq, static_cast<const T*>(a.q) + r * a.qs.row, a.qs,
-                                static_cast<T*>(a.q_out) + r * a.qo.row, a.qo, cs[warp]);
+  if ((int)blockIdx.x >= a.page_blocks) {
+    turn_queries<T, DQK, Fast>(a, cs[0] + warp * kQueryRows);
     return;
   }
   const int count = *a.plan.count + 1;
-  const int first = blockIdx.x - a.q_blocks, step = gridDim.x - a.q_blocks;
+  const int first = blockIdx.x, step = a.page_blocks;
   bool bad = false;
 
-  // One page by the whole CTA, its rows in `rows[0]`; `ahead` runs behind the
-  // first loads.  A warp takes K and V of every kWarps-th head in turn, the
-  // next block's loads before the work on the last.
-  auto dense = [&](int page, auto&& ahead) {
+  auto page_of = [&](int at) {  // -1: a plan of another pool
+    const int page = a.plan.keys[at];
+    return page < c.num_pages ? page : -1;
+  };
+  // One page by the whole CTA, its rows in rows[now], K's first blocks loaded
+  // in k and their turns to be put in cs[side].  A warp takes K and V of
+  // every kWarps-th head in turn, each block's loads before the work on the
+  // last; `ahead` runs behind the first loads, and what it puts in the other
+  // buffers is there for `next`, which runs before the last V block's work.
+  auto dense = [&](int page, int now, int side, KBlock<T, DQK, Fast>& k, auto&& ahead, auto&& next) {
     uint8_t *kb = c.data + page * c.page_stride, *vb = kb + c.v_offset, *scales = c.scales + page * c.scale_stride;
-    KBlock<T, DQK, Fast> k;
     VBlock<T, DV, Fast> v;
     int h = warp;
-    if (h < a.H) k.load(a, rows[0], h, scales + h);
+    if (h < a.H) v.load(a, rows[now], h, scales + a.H + h);
     ahead();
-    fill_turns(a.rot, rows[0], cs);
+    fill_turns(a.rot, rows[now], cs[side]);
     __syncthreads();
     for (; h < a.H; h += kWarps) {
-      v.load(a, rows[0], h, scales + a.H + h);
-      k.put(a, rows[0], cs, kb + (int64_t)h * kTok * DQK, scales + h, bad);
-      if (h + kWarps < a.H) k.load(a, rows[0], h + kWarps, scales + h + kWarps);
-      v.put(a, rows[0], vb + (int64_t)h * kTok * DV, scales + a.H + h, bad);
+      k.put(a, rows[now], cs[side], kb + (int64_t)h * kTok * DQK, scales + h, bad);
+      const bool more = h + kWarps < a.H;
+      if (more)
+        k.load(a, rows[now], h + kWarps, scales + h + kWarps);
+      else
+        next();
+      v.put(a, rows[now], vb + (int64_t)h * kTok * DV, scales + a.H + h, bad);
+      if (more) v.load(a, rows[now], h + kWarps, scales + a.H + h + kWarps);
     }
-    __syncthreads();
+    if (warp >= a.H) next();
   };
 
   if (2 * (int64_t)count <= a.n) {
-    // Dense: the next page's rows are fetched behind this one's first loads.
-    int page = -1, r = -1;
-    auto fetch = [&](int e) {
-      page = -1;
-      if (e >= count) return;
+    // Dense.  Three buffers of rows and two of turns: while the slowest warp is
+    // at one page's, the fastest has come to write the rows after the next and
+    // the turns of the next.
+    int e = first, now = 0, side = 0, page = -1;
+    if (e >= count) return;
+    {
       const int at = a.plan.list[e];
-      page = a.plan.keys[at];
-      if (page >= c.num_pages) page = -1;  // a plan of another pool
-      if (threadIdx.x < kTok) r = a.plan.rows[(size_t)at * kTok + threadIdx.x];
+      page = page_of(at);
+      if (threadIdx.x < kTok) rows[0][threadIdx.x] = page < 0 ? -1 : a.plan.rows[(size_t)at * kTok + threadIdx.x];
+    }
+    __syncthreads();
+    KBlock<T, DQK, Fast> k;
+    auto load_k = [&](int buf, int pg) {
+      if (warp < a.H) k.load(a, rows[buf], warp, c.scales + max(pg, 0) * c.scale_stride + warp);
     };
-    fetch(first);
-    for (int e = first; e < count; e += step) {
-      const int now = page;
-      if (threadIdx.x < kTok) rows[0][threadIdx.x] = now < 0 ? -1 : r;
-      __syncthreads();
-      if (now >= 0)
-        dense(now, [&] { fetch(e + step); });
-      else
-        fetch(e + step);
+    load_k(0, page);
+    for (; e < count; e += step) {
+      const int after = now == 2 ? 0 : now + 1;
+      int next_page = -1;
+      auto ahead = [&] {
+        if (e + step < count) {
+          const int at = a.plan.list[e + step];
+          next_page = page_of(at);
+          if (threadIdx.x < kTok)
+            rows[after][threadIdx.x] = next_page < 0 ? -1 : a.plan.rows[(size_t)at * kTok + threadIdx.x];
+        }
+      };
+      auto next = [&] {
+        if (e + step < count) load_k(after, next_page);
+      };
+      dense(max(page, 0), now, side, k, ahead, next);  // (no rows of a page of another pool)
+      page = next_page;
+      now = after;
+      side ^= 1;
     }
   } else {
     for (int e0 = first * kSparse; e0 < count; e0 += step * kSparse) {
@@ -737,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, append_ctas(sizeof(T), DQK > DV ? DQ
       if (live == 1) {  // one of the page's warps takes K, the other V
         uint8_t *kb = c.data + page * c.page_stride, *scales = c.scales + page * c.scale_stride;
         if (warp % 2 == 0)
-          one_k8<T, DQK, Fast>(a, r, tok, kb, scales, cs[warp], bad);
+          one_k8<T, DQK, Fast>(a, r, tok, kb, scales, cs[0][warp], bad);
         else
           one_v8<T, DV, Fast>(a, r, tok, kb + c.v_offset, scales + a.H, bad);
       }
@@ -748,10 +814,12 @@ __global__ void __launch_bounds__(kThreads, append_ctas(sizeof(T), DQK > DV ? DQ
           if (warp == 2 * i && lane == 0) rows[1][0] = live > 1 ? page : -1;
           __syncthreads();
           const int now = rows[1][0];
-          if (now >= 0)
-            dense(now, [] {});
-          else
-            __syncthreads();
+          if (now >= 0) {
+            KBlock<T, DQK, Fast> k;
+            if (warp < a.H) k.load(a, rows[0], warp, c.scales + now * c.scale_stride + warp);
+            dense(now, 0, 0, k, [] {}, [] {});
+          }
+          __syncthreads();
         }
       }
     }
@@ -763,25 +831,28 @@ __global__ void __launch_bounds__(kThreads, append_ctas(sizeof(T), DQK > DV ? DQ
 // for any head sizes and alignments.
 template <typename T, typename TP, int D>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, PoolGeom g, TP* pool, int layer) {
-  __shared__ __align__(16) float2 cs[kWarps][kMaxPairs];
+  __shared__ __align__(16) float2 cs[kWarps * kQueryRows][kMaxPairs];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if ((int)blockIdx.x < a.q_blocks) {
-    const int64_t r = query_row(a);
-    if (r < 0) return;
-    const T* src = static_cast<const T*>(a.q) + r * a.qs.row;
-    T* dst = static_cast<T*>(a.q_out) + r * a.qo.row;
-    if constexpr (D > 0)
-      turn_row<T, T, D, true>(a.rot, r, a.Hq, src, a.qs, dst, a.qo, cs[warp]);
-    else
-      turn_row_any<T, T>(a.rot, r, a.Hq, a.dqk, src, a.qs, dst, a.qo, cs[warp]);
+  if ((int)blockIdx.x >= a.page_blocks) {
+    if constexpr (D > 0) {
+      turn_queries<T, D, true>(a, cs + warp * kQueryRows);
+    } else {
+      uint32_t live;
+      const int64_t r0 = query_rows(a, &live);
+      for (; live; live &= live - 1) {
+        const int64_t r = r0 + __ffs(live) - 1;
+        turn_row_any<T, T>(a.rot, r, a.Hq, a.dqk, static_cast<const T*>(a.q) + r * a.qs.row, a.qs,
+                           static_cast<T*>(a.q_out) + r * a.qo.row, a.qo, cs[warp * kQueryRows]);
+      }
+    }
     return;
   }
   const int count = *a.plan.count + 1;
   const Strides ks{0, (int64_t)kTok * g.dqk, 1};
-  const int64_t step = (int64_t)(gridDim.x - a.q_blocks) * kWarps;
-  for (int64_t u = (int64_t)(blockIdx.x - a.q_blocks) * kWarps + warp; u < (int64_t)count * kTok; u += step) {
+  const int64_t step = (int64_t)a.page_blocks * kWarps;
+  for (int64_t u = (int64_t)blockIdx.x * kWarps + warp; u < (int64_t)count * kTok; u += step) {
     const int at = a.plan.list[u / kTok];
     const int r = a.plan.rows[(size_t)at * kTok + u % kTok];
     const int64_t slot = (int64_t)a.plan.keys[at] * kTok + u % kTok;
@@ -799,7 +870,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, PoolGeom
         raw.get(x);
         store8(vo + (int64_t)h * kTok * g.dv + e, x);
       }
-      turn_row<T, TP, D, true>(a.rot, r, a.H, k, a.ks, ko, ks, cs[warp]);
+      turn_rows<1, T, TP, D, true>(a.rot, r, 1, a.H, static_cast<const T*>(a.k), a.ks,
+                                   [&](int64_t) { return ko; }, ks, cs + warp);
     } else {
       turn_row_any<T, TP>(a.rot, r, a.H, g.dqk, k, a.ks, ko, ks, cs[warp]);
       for (int i = lane; i < a.H * g.dv; i += 32)
@@ -859,11 +931,18 @@ imba_status_t launch_append(const imba_cache_desc& c, const imba_pool_desc& pool
   a.slots = d.slots;
   a.status = d.status;
   a.num_slots = pool.num_pages * kTok;
-  a.q_blocks = a.Hq ? (d.num_rows + kWarps - 1) / kWarps : 0;
+  // A row of few heads is one or two passes of a warp: several rows then keep
+  // its loads in flight (57k rows of 8 heads of 64 84 us with four, 98 with one;
+  // rows of 32 heads of 128 274 and 250), if the SMs stay full.
+  a.q_rows = d.num_rows >= 148 * 2 * kWarps * kQueryRows && a.Hq * c.attention_dim <= 1024 ? kQueryRows : 1;
+  const int64_t q_blocks = a.Hq ? (d.num_rows + kWarps * a.q_rows - 1) / (kWarps * a.q_rows) : 0;
   cudaError_t e = cudaErrorInvalidValue;
   if (c.dtype == IMBA_DTYPE_E4M3) {
-    // a page a CTA with two tokens or more in it on average, else kSparse
-    const dim3 grid((unsigned)(a.q_blocks + std::min<int64_t>((d.num_rows + 1) / 2, 148 * 4)));
+    // a page a CTA with two tokens or more in it on average, else kSparse;
+    // as many CTAs as there is room for, which go from page to page
+    const int ctas = append_ctas(sizeof(T), std::max(c.attention_dim, c.linear_dim));
+    a.page_blocks = (int)std::min<int64_t>((d.num_rows + 1) / 2, 148 * ctas);
+    const dim3 grid((unsigned)(q_blocks + a.page_blocks));
     const Cache8 l = cache8_layer(c, pool, d.layer);
 #define IMBA_APPEND8(DQK, DV) \
   if (c.attention_dim == DQK && c.linear_dim == DV) e = launch_append8<T, DQK, DV>(grid, a, l, fast, s);
@@ -876,7 +955,8 @@ imba_status_t launch_append(const imba_cache_desc& c, const imba_pool_desc& pool
 #undef IMBA_APPEND8
   } else {
     const PoolGeom g = cache_geom(c, pool.num_pages);
-    const dim3 grid((unsigned)(a.q_blocks + std::min<int64_t>(d.num_rows, 148 * 8)));
+    a.page_blocks = (int)std::min<int64_t>(d.num_rows, 148 * 8);
+    const dim3 grid((unsigned)(q_blocks + a.page_blocks));
     e = c.dtype == IMBA_DTYPE_BF16 ? launch_append_full<T, bf16>(grid, a, g, pool.base, d.layer, fast, s)
                                    : launch_append_full<T, float>(grid, a, g, pool.base, d.layer, fast, s);
   }
