@@ -40,6 +40,7 @@ FLAG_SIMT_GEMM = 1
 FLAG_SIMT_ATTN = 2
 FLAG_SIMT_BOARD = 4
 SIMT_FLAGS = {"gemm": FLAG_SIMT_GEMM, "attn": FLAG_SIMT_ATTN, "board": FLAG_SIMT_BOARD}
+FLAG_CACHE_E4M3 = 8  # the handle's KV pool is in 8 bits
 MAX_LAYERS = 32
 PAGE_TOKENS = 16
 NOALLOC_SCRATCH_BYTES = 8 << 20

@@ -9,6 +9,8 @@
 #include <new>
 #include <type_traits>
 
+#include "attend8.cuh"
+#include "cache_plan.cuh"
 #include "gemm_tc.cuh"
 #include "kernels.cuh"
 
@@ -50,6 +52,12 @@ size_t workspace_layout(const imba_model* m, int32_t rows, void* base, Workspace
   w.recs = static_cast<int*>(take(d.dtype == IMBA_DTYPE_BF16 ? 2 * R * kAttnRecInts * sizeof(int) : 0));
   // per row and head (max, sum) of the paged attention's pages-only pass
   w.ml = static_cast<float2*>(take(d.dtype == IMBA_DTYPE_BF16 ? R * d.num_heads * sizeof(float2) : 0));
+  const size_t tiles = (R + IMBA_PAGE_TOKENS - 1) / IMBA_PAGE_TOKENS;
+  w.kv = take(m->cache8 ? tiles * IMBA_PAGE_TOKENS * (hdq + hdv) * eb : 0);
+  w.kv_slots = static_cast<int*>(take(m->cache8 ? R * sizeof(int) : 0));
+  w.append_bytes = m->cache8 ? imba_append_plan_bytes((int32_t)R) : 0;
+  w.append_plan = take(w.append_bytes);
+  w.attend_plan = take(m->cache8 ? attend_step_bytes(m->cache(), (int32_t)R) : 0);
   w.bytes = off;
   if (ws) *ws = w;
   return off;
@@ -65,7 +73,7 @@ imba_status_t validate_desc(const imba_model_desc* d) {
   if ((int64_t)d->num_heads * d->linear_dim > 1024) return IMBA_ERR_UNSUPPORTED;
   if (d->vocab <= 0 || d->max_pos <= 0 || d->halfmove_vocab <= 0 || d->fullmove_vocab <= 0) return IMBA_ERR_ARG;
   if (d->dtype != IMBA_DTYPE_F32 && d->dtype != IMBA_DTYPE_BF16) return IMBA_ERR_ARG;
-  if (d->flags & ~(IMBA_FLAG_SIMT_GEMM | IMBA_FLAG_SIMT_ATTN | IMBA_FLAG_SIMT_BOARD)) return IMBA_ERR_ARG;
+  if (d->flags & ~(IMBA_FLAG_SIMT_GEMM | IMBA_FLAG_SIMT_ATTN | IMBA_FLAG_SIMT_BOARD | IMBA_FLAG_CACHE_E4M3)) return IMBA_ERR_ARG;
   const void* req[] = {d->piece_square, d->board_params, d->board_out_w, d->board_out_b, d->emb_seq,
                        d->emb_turn,     d->emb_castle,   d->emb_ep,      d->emb_halfmove, d->emb_fullmove,
                        d->emb_prev_move, d->emb_pos,     d->final_norm_w, d->final_norm_b, d->policy_w,
@@ -81,13 +89,13 @@ imba_status_t validate_desc(const imba_model_desc* d) {
 // Shapes the bf16 tensor-core kernels cover: the GEMM tiles (d and H dv
 // multiples of 128, the uvqk width a multiple of 256) and the paged
 // attention (head dims 64 / 64, at most 16 head groups of 8).
-bool bf16_shape_supported(const imba_model_desc& d, bool simt_gemm, bool simt_attn) {
+bool bf16_shape_supported(const imba_model_desc& d, bool simt_gemm, bool other_attn) {
   const int hdv = d.num_heads * d.linear_dim;
   const int uvqk_n = 2 * d.num_heads * (d.linear_dim + d.attention_dim);
   const bool gemm_ok = d.model_dim % 128 == 0 && hdv % 128 == 0 && uvqk_n % 256 == 0 && d.attention_dim % 32 == 0 &&
                        d.linear_dim % 32 == 0;
   const bool attn_ok = d.attention_dim == 64 && d.linear_dim == 64 && d.num_heads <= 128;
-  return (simt_gemm || gemm_ok) && (simt_attn || attn_ok);
+  return (simt_gemm || gemm_ok) && (other_attn || attn_ok);
 }
 
 imba_status_t validate_step(const imba_model* m, const imba_step_desc* st, const imba_pool_desc* pool) {
@@ -112,6 +120,91 @@ imba_status_t validate_step(const imba_model* m, const imba_step_desc* st, const
   if ((st->legal_logits || st->legal_logprob) && !st->legal_off) return IMBA_ERR_ARG;
   (void)m;
   return IMBA_OK;
+}
+
+// Pools in 8 bits: head dims that their kernels take, and for bf16 handles
+// the width of the gate pass on bf16 attention outputs.
+bool cache8_supported(const imba_model_desc& d) {
+  return cache8_dims_ok(d.attention_dim, d.linear_dim) &&
+         (d.dtype != IMBA_DTYPE_BF16 || d.num_heads * d.linear_dim % 128 == 0);
+}
+
+__global__ void count_kernel(int* out, int n) {
+  pdl_wait();
+  pdl_trigger();
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n) out[i] = i;
+}
+
+// A step over a pool in 8 bits: what every layer's append and attention share.
+struct Cache8Step {
+  imba_cache_desc cache;
+  PoolGeom staged;  // of w.kv
+  imba_append_desc append;
+  AttendArgs attend;
+  int64_t tile;
+};
+
+template <typename T>
+cudaError_t begin_cache8(const imba_model* m, const imba_step_desc& st, const imba_pool_desc& pool, Workspace& w,
+                         Cache8Step* c, cudaStream_t s) {
+  const imba_model_desc& md = m->d;
+  c->cache = m->cache();
+  imba_cache_desc one = c->cache;
+  one.num_layers = 1;
+  const int tiles = (st.num_rows + IMBA_PAGE_TOKENS - 1) / IMBA_PAGE_TOKENS;
+  c->staged = cache_geom(one, tiles);
+  c->tile = c->staged.page_stride;
+  imba_append_desc& a = c->append = {};
+  a.num_rows = st.num_rows;
+  a.src_dtype = md.dtype;
+  a.slots = st.row_dst_slot;
+  a.k = w.kv;
+  a.v = static_cast<T*>(w.kv) + c->staged.v_offset;
+  const int64_t ks[3] = {md.attention_dim, (int64_t)IMBA_PAGE_TOKENS * md.attention_dim, 1};
+  const int64_t vs[3] = {md.linear_dim, (int64_t)IMBA_PAGE_TOKENS * md.linear_dim, 1};
+  for (int i = 0; i < 3; ++i) {
+    a.k_stride[i] = ks[i];
+    a.v_stride[i] = vs[i];
+  }
+  a.status = st.status;
+  cudaError_t e = launch_pdl(count_kernel, dim3((st.num_rows + 255) / 256), dim3(256), 0, s, w.kv_slots, st.num_rows);
+  if (e != cudaSuccess) return e;
+  e = launch_append_plan(pool.num_pages * IMBA_PAGE_TOKENS, st.num_rows, st.row_dst_slot, w.append_plan, st.status, s);
+  if (e != cudaSuccess) return e;
+  AttendArgs& t = c->attend;
+  t.rows = {};
+  t.rows.num_rows = st.num_rows;
+  t.rows.num_segs = st.num_chunks;
+  t.rows.num_groups = st.num_groups;
+  t.rows.num_group_pages = st.num_group_pages;
+  t.rows.num_extra = st.num_extra;
+  t.rows.num_q_heads = md.num_heads;
+  t.rows.seg_group = st.chunk_group;
+  t.rows.seg_row_off = st.chunk_row_off;
+  t.rows.seg_nrows = st.chunk_nrows;
+  t.rows.row_perm = st.row_perm;
+  t.rows.row_vis = st.row_vis;
+  t.rows.positions = st.positions;
+  t.rows.group_page_off = st.group_page_off;
+  t.rows.group_pages = st.group_pages;
+  t.rows.row_extra_off = st.row_extra_off;
+  t.rows.extra_slot = st.extra_slot;
+  t.rows.extra_pos = st.extra_pos;
+  t.rows.status = st.status;
+  t.shape = attend_shape(c->cache, t.rows, attend_step_most(st.num_rows));
+  t.plan = attend_plan_view(c->cache, t.rows, t.shape, w.attend_plan);
+  t.call = {};
+  t.call.dtype = md.dtype;
+  t.call.q = w.q;
+  t.call.out = w.attn;
+  t.call.q_stride[0] = (int64_t)md.num_heads * md.attention_dim;
+  t.call.q_stride[1] = md.attention_dim;
+  t.call.out_stride[0] = (int64_t)md.num_heads * md.linear_dim;
+  t.call.out_stride[1] = md.linear_dim;
+  t.call.scale = 1.0f / sqrtf((float)md.attention_dim);
+  t.call.max_pos = md.max_pos;
+  return st.num_chunks ? launch_attend_plan(c->cache, t.rows, t.shape, t.plan, s) : cudaSuccess;
 }
 
 // Records phase-boundary events when profiling; a no-op otherwise.
@@ -144,7 +237,9 @@ imba_status_t run_step(const imba_model* m, const imba_step_desc& st, const imba
   IMBA_CK(pm.mark(s));
   IMBA_CK(cudaMemsetAsync(w.counters, 0, kNumCounters * sizeof(int), s));
   // The paged attention's work items, resolved once for every layer.
-  const bool paged_attn = md.dtype == IMBA_DTYPE_BF16 && !m->simt_attn;
+  const bool paged_attn = md.dtype == IMBA_DTYPE_BF16 && !m->simt_attn && !m->cache8;
+  Cache8Step c8;
+  if (m->cache8) IMBA_CK(begin_cache8<T>(m, st, pool, w, &c8, s));
   if (paged_attn) IMBA_CK(launch_attn_items(st, g, w.recs, s));
   // A step whose rows find every key in their groups' pages and that has
   // several rows per group on average (a jagged prefill of documents) runs
@@ -184,7 +279,14 @@ imba_status_t run_step(const imba_model* m, const imba_step_desc& st, const imba
   for (int l = 0; l < md.num_layers; ++l) {
     IMBA_CK(launch_ln_rows<T>(w.x, R, d, 1e-6f, static_cast<T*>(w.xn), s));
     IMBA_CK(pm.mark(s));
+    // (a pool in 8 bits gets the layer's keys and values from the workspace)
     EpiUVQK<T> epi{static_cast<T*>(w.u), static_cast<T*>(w.q), poolp, st.row_dst_slot, g, l, st.status};
+    if (m->cache8) {
+      epi.pool = static_cast<T*>(w.kv);
+      epi.dst_slot = w.kv_slots;
+      epi.g = c8.staged;
+      epi.layer = 0;
+    }
     if (!gemm_tc_launch_uvqk(m, l, R, static_cast<const T*>(w.xn), epi, s, &e)) {
       if (tc_gemm) return IMBA_ERR_UNSUPPORTED;
       IMBA_CK(launch_gemm_simt<T, T, EpiUVQK<T>>(static_cast<const T*>(w.xn), d,
@@ -192,13 +294,24 @@ imba_status_t run_step(const imba_model* m, const imba_step_desc& st, const imba
     } else if (e != cudaSuccess) {
       return IMBA_ERR_CUDA;
     }
+    if (m->cache8) {
+      c8.append.layer = l;
+      const imba_status_t ap = launch_append<T>(c8.cache, pool, c8.append, w.append_plan, s, c8.tile, c8.tile);
+      if (ap != IMBA_OK) return ap;
+    }
     IMBA_CK(pm.mark(s));
     AttnArgs aa{w.q, pool.base, g, l, md.ps_w[l], md.max_pos, 1.0f / sqrtf((float)md.attention_dim), st, w.attn,
                 w.counters + l * kCountersPerLayer};
     bool fused = false;
     bf16* gated_bf = std::is_same<T, bf16>::value ? reinterpret_cast<bf16*>(w.gated) : nullptr;
     bool gate_bf16 = false;  // the attention output was stored as bf16
-    if (prefill_attn && launch_attn_prefill(aa, md.num_layers, pool.num_pages, w.recs, s, &e)) {
+    if (m->cache8) {
+      c8.attend.cache = cache8_layer(c8.cache, pool, l);
+      c8.attend.call.layer = l;
+      c8.attend.call.bias = md.ps_w[l];
+      if (st.num_chunks) IMBA_CK(launch_attend8<T>(c8.cache, c8.attend, s));
+      gate_bf16 = std::is_same<T, bf16>::value;
+    } else if (prefill_attn && launch_attn_prefill(aa, md.num_layers, pool.num_pages, w.recs, s, &e)) {
       if (e != cudaSuccess) return IMBA_ERR_CUDA;
       gate_bf16 = true;
     } else if (partial_attn && launch_attn_page(aa, md.num_layers, md, pool.num_pages,
@@ -313,7 +426,10 @@ imba_status_t imba_model_create(const imba_model_desc* desc, imba_model** out) {
   m->simt_gemm = (desc->flags & IMBA_FLAG_SIMT_GEMM) != 0;
   m->simt_attn = (desc->flags & IMBA_FLAG_SIMT_ATTN) != 0;
   m->simt_board = (desc->flags & IMBA_FLAG_SIMT_BOARD) != 0;
-  if (desc->dtype == IMBA_DTYPE_BF16 && !imba::bf16_shape_supported(*desc, m->simt_gemm, m->simt_attn)) {
+  m->cache8 = (desc->flags & IMBA_FLAG_CACHE_E4M3) != 0;
+  if ((m->cache8 && !imba::cache8_supported(*desc)) ||
+      (desc->dtype == IMBA_DTYPE_BF16 &&
+       !imba::bf16_shape_supported(*desc, m->simt_gemm, m->simt_attn || m->cache8))) {
     delete m;
     return IMBA_ERR_UNSUPPORTED;
   }
@@ -398,6 +514,11 @@ static imba_status_t kv_copy(const imba_model* model, const imba_pool_desc* pool
   if (layer < 0 || layer >= model->d.num_layers || n < 0) return IMBA_ERR_RANGE;
   if (n == 0) return IMBA_OK;
   if (!slots || !dk || !dv) return IMBA_ERR_ARG;
+  if (model->cache8) {
+    if (to_pool) return IMBA_ERR_UNSUPPORTED;
+    const imba_cache_desc c = model->cache();
+    return imba_kv_read(&c, pool, layer, n, slots, model->d.dtype, dk, dv, status, stream);
+  }
   const imba::PoolGeom g = model->geom(pool->num_pages);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
@@ -425,6 +546,7 @@ imba_status_t imba_kv_scatter_indexed(const imba_model* model, const imba_pool_d
   if (layer < 0 || layer >= model->d.num_layers || n < 0) return IMBA_ERR_RANGE;
   if (n == 0) return IMBA_OK;
   if (!slots || !src_a || !src_b || !src_k || !src_v || !strides_k || !strides_v) return IMBA_ERR_ARG;
+  if (model->cache8) return IMBA_ERR_UNSUPPORTED;
   imba::KVStrides st;
   for (int i = 0; i < 4; ++i) {
     st.k[i] = strides_k[i];

@@ -56,7 +56,12 @@ struct AttendPlan {
   size_t bytes;
 };
 
-AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r);
+// most: items that splitting may add at most (an imba_step's workspace is
+// sized by its rows alone).
+AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r, int64_t most = INT64_MAX);
+// The largest plan of a step of `rows` rows, with most = attend_step_most(rows).
+inline int64_t attend_step_most(int64_t rows) { return rows + 8; }
+size_t attend_step_bytes(const imba_cache_desc& c, int32_t rows);
 AttendPlan attend_plan_view(const imba_cache_desc& c, const imba_attend_desc& r, const AttendShape& sh, void* base);
 
 struct AttendArgs {
@@ -69,6 +74,8 @@ struct AttendArgs {
 
 template <typename T>
 cudaError_t launch_attend8(const imba_cache_desc& c, const AttendArgs& a, cudaStream_t s);
+cudaError_t launch_attend_plan(const imba_cache_desc& c, const imba_attend_desc& r, const AttendShape& sh,
+                               const AttendPlan& p, cudaStream_t s);
 imba_status_t validate_cache(const imba_cache_desc* c);
 imba_status_t validate_pool(const imba_pool_desc* pool);
 

@@ -194,29 +194,52 @@ __global__ void attend_rows_kernel(imba_attend_desc r, AttendShape sh, AttendPla
 
 }  // namespace
 
-AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r) {
+namespace {
+
+// The shape with tiles of 8 rt rows and `warps` warps a unit.
+AttendShape shape_of(const imba_cache_desc& c, const imba_attend_desc& r, int rt, int warps, int64_t most) {
   AttendShape sh;
   sh.share = r.num_q_heads / c.num_heads;
+  sh.rt = rt;
+  sh.tile_rows = kTileRows * rt;
   const int64_t flat = (int64_t)r.num_rows * sh.share;
-  // Rows of a tile by what a segment has on average.
-  const int64_t per_seg = r.num_segs ? (flat + r.num_segs - 1) / r.num_segs : 0;
-  sh.rt = per_seg <= 8 ? 1 : 2;
-  sh.tile_rows = kTileRows * sh.rt;
   const int64_t tiles = r.num_segs ? (flat + sh.tile_rows - 1) / sh.tile_rows + r.num_segs : 0;
   sh.max_tiles = (int)std::min<int64_t>(tiles, INT32_MAX);
-  // One warp per unit when there are enough units to fill the device and the
-  // page lists are short on average; else the CTA's warps share a unit.
-  const int64_t avg = r.num_groups ? r.num_group_pages / r.num_groups : 0;
-  const int64_t busy = std::max<int64_t>(1, flat / sh.tile_rows) * c.num_heads;
-  sh.warps = std::max<int64_t>(busy, (int64_t)r.num_segs * c.num_heads) >= 148 * 8 && avg <= 32 ? 1 : kUnitWarps;
-  sh.min_pages = sh.warps == 1 ? 16 : 8;
+  sh.warps = warps;
+  sh.min_pages = warps == 1 ? 16 : 8;
   // About four CTAs' worth of units for each that is resident.
-  sh.target = std::max(1, 148 * 2 * 4 * (kUnitWarps / sh.warps) / c.num_heads);
+  sh.target = (int)std::min<int64_t>(most, std::max(1, 148 * 2 * 4 * (kUnitWarps / warps) / c.num_heads));
   const int64_t by_len = (int64_t)sh.max_tiles * ((r.num_group_pages + sh.min_pages - 1) / sh.min_pages);
   const int64_t cut = std::min<int64_t>(by_len, sh.target);  // full-size items; each tile may add one smaller
   sh.max_items = (int)std::min<int64_t>(sh.max_tiles + cut, INT32_MAX / 4);
   sh.max_parts = (int)std::min<int64_t>(2 * cut, INT32_MAX / 4);
   return sh;
+}
+
+}  // namespace
+
+AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r, int64_t most) {
+  const int64_t flat = (int64_t)r.num_rows * (r.num_q_heads / c.num_heads);
+  // Rows of a tile by what a segment has on average.
+  const int64_t per_seg = r.num_segs ? (flat + r.num_segs - 1) / r.num_segs : 0;
+  const int rt = per_seg <= 8 ? 1 : 2;
+  // One warp per unit when there are enough units to fill the device and the
+  // page lists are short on average; else the CTA's warps share a unit.
+  const int64_t avg = r.num_groups ? r.num_group_pages / r.num_groups : 0;
+  const int64_t busy = std::max<int64_t>(flat / (kTileRows * rt), r.num_segs) * c.num_heads;
+  return shape_of(c, r, rt, busy >= 148 * 8 && avg <= 32 ? 1 : kUnitWarps, most);
+}
+
+size_t attend_step_bytes(const imba_cache_desc& c, int32_t rows) {
+  imba_attend_desc r = {};
+  r.num_rows = r.num_segs = r.num_groups = rows;  // every chunk holds a row
+  r.num_group_pages = INT32_MAX / IMBA_PAGE_TOKENS;
+  r.num_q_heads = c.num_heads;
+  size_t most = 0;
+  for (int rt = 1; rt <= 2; ++rt)
+    for (int warps : {1, kUnitWarps})
+      most = std::max(most, attend_plan_view(c, r, shape_of(c, r, rt, warps, attend_step_most(rows)), nullptr).bytes);
+  return most;
 }
 
 AttendPlan attend_plan_view(const imba_cache_desc& c, const imba_attend_desc& r, const AttendShape& sh, void* base) {
@@ -238,6 +261,15 @@ AttendPlan attend_plan_view(const imba_cache_desc& c, const imba_attend_desc& r,
   p.o = static_cast<float*>(take((size_t)sh.max_parts * c.num_heads * sh.tile_rows * c.linear_dim * sizeof(float)));
   p.bytes = off;
   return p;
+}
+
+cudaError_t launch_attend_plan(const imba_cache_desc& c, const imba_attend_desc& r, const AttendShape& sh,
+                               const AttendPlan& p, cudaStream_t s) {
+  const cudaError_t e =
+      launch_pdl(attend_items_kernel, dim3(1), dim3(kPlanThreads), 0, s, r, sh, p, (int)c.num_heads);
+  if (e != cudaSuccess) return e;
+  const int64_t blocks = ((int64_t)sh.max_tiles * sh.tile_rows + 255) / 256;
+  return launch_pdl(attend_rows_kernel, dim3((unsigned)std::min<int64_t>(blocks, 148 * 8)), dim3(256), 0, s, r, sh, p);
 }
 
 namespace {
@@ -290,13 +322,7 @@ imba_status_t imba_attend_plan(const imba_cache_desc* cache, const imba_pool_des
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const imba::AttendShape sh = imba::attend_shape(*cache, *rows);
   const imba::AttendPlan p = imba::attend_plan_view(*cache, *rows, sh, plan);
-  cudaError_t e = imba::launch_pdl(imba::attend_items_kernel, dim3(1), dim3(imba::kPlanThreads), 0, s, *rows, sh, p,
-                                   (int)cache->num_heads);
-  if (e != cudaSuccess) return IMBA_ERR_CUDA;
-  const int64_t blocks = ((int64_t)sh.max_tiles * sh.tile_rows + 255) / 256;
-  e = imba::launch_pdl(imba::attend_rows_kernel, dim3((unsigned)std::min<int64_t>(blocks, 148 * 8)), dim3(256), 0, s,
-                       *rows, sh, p);
-  return e == cudaSuccess ? IMBA_OK : IMBA_ERR_CUDA;
+  return imba::launch_attend_plan(*cache, *rows, sh, p, s) == cudaSuccess ? IMBA_OK : IMBA_ERR_CUDA;
 }
 
 imba_status_t imba_attend(const imba_cache_desc* cache, const imba_pool_desc* pool, const imba_attend_desc* rows,

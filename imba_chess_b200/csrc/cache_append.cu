@@ -62,6 +62,16 @@ __global__ void read8_kernel(Cache8 c, int dqk, int dv, int n, const int32_t* __
 
 }  // namespace
 
+cudaError_t launch_append_plan(int64_t num_slots, int32_t num_rows, const int32_t* slots, void* plan, int32_t* status,
+                               cudaStream_t s) {
+  const PlanView pv = plan_view(plan, num_rows);
+  const size_t clear = (size_t)(kPlanHead + (int64_t)pv.cap * (1 + kTok)) * sizeof(int32_t);
+  const cudaError_t e = cudaMemsetAsync(plan, 0xff, clear, s);
+  if (e != cudaSuccess || num_rows == 0) return e;
+  return launch_pdl(append_plan_kernel, dim3((num_rows + 127) / 128), dim3(128), 0, s, pv, (int)num_rows, slots,
+                    num_slots, status);
+}
+
 imba_status_t validate_cache(const imba_cache_desc* c) {
   if (!c) return IMBA_ERR_ARG;
   if (c->num_layers <= 0 || c->num_heads <= 0 || c->attention_dim <= 0 || c->linear_dim <= 0) return IMBA_ERR_ARG;
@@ -108,12 +118,8 @@ imba_status_t imba_append_plan(const imba_pool_desc* pool, int32_t num_rows, con
   if (!plan || (num_rows > 0 && !slots) || (reinterpret_cast<uintptr_t>(plan) & 255)) return IMBA_ERR_ARG;
   if (plan_bytes < imba_append_plan_bytes(num_rows)) return IMBA_ERR_OOM;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const imba::PlanView pv = imba::plan_view(plan, num_rows);
-  const size_t clear = (size_t)(imba::kPlanHead + (int64_t)pv.cap * (1 + IMBA_PAGE_TOKENS)) * sizeof(int32_t);
-  if (cudaMemsetAsync(plan, 0xff, clear, s) != cudaSuccess) return IMBA_ERR_CUDA;
-  if (num_rows == 0) return IMBA_OK;
-  const cudaError_t e = imba::launch_pdl(imba::append_plan_kernel, dim3((num_rows + 127) / 128), dim3(128), 0, s, pv,
-                                         (int)num_rows, slots, pool->num_pages * IMBA_PAGE_TOKENS, status);
+  const cudaError_t e =
+      imba::launch_append_plan(pool->num_pages * IMBA_PAGE_TOKENS, num_rows, slots, plan, status, s);
   return e == cudaSuccess ? IMBA_OK : IMBA_ERR_CUDA;
 }
 

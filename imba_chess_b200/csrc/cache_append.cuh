@@ -30,7 +30,10 @@ namespace imba {
 namespace {
 
 struct Strides {
-  int64_t row, head, elem;
+  int64_t tile, row, head, elem;
+  // Row r's first element; rows come in tiles of 16 (a step's staged keys and
+  // values lie like a pool's pages), tile = 16 row when they are evenly apart.
+  __device__ __forceinline__ int64_t at(int64_t r) const { return (r >> 4) * tile + (r & 15) * row; }
 };
 
 struct AppendArgs {
@@ -290,7 +293,7 @@ __device__ __forceinline__ void turn_rows(const imba_rotary_desc& rot, int64_t r
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       int row, h;
-      if (place(i, &row, &h)) raw[i].load(src + (r0 + row) * ss.row + h * ss.head, ss, m, p0);
+      if (place(i, &row, &h)) raw[i].load(src + ss.at(r0 + row) + h * ss.head, ss, m, p0);
     }
     if (!filled) {  // behind the first loads
       __syncwarp();  // the last rows' are done with
@@ -359,7 +362,7 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, float2 (*cs)[k
   uint32_t live;
   const int64_t r0 = query_rows(a, &live);
   if (!live) return;
-  auto dst = [&](int64_t r) { return static_cast<T*>(a.q_out) + r * a.qo.row; };
+  auto dst = [&](int64_t r) { return static_cast<T*>(a.q_out) + a.qo.at(r); };
   if (a.q_rows == 1)
     turn_rows<1, T, T, D, Fast>(a.rot, r0, live, a.Hq, static_cast<const T*>(a.q), a.qs, dst, a.qo, cs);
   else
@@ -460,7 +463,7 @@ struct KBlock {
       if (r < 0)
         raw[i].zero();
       else
-        raw[i].load(static_cast<const T*>(a.k) + r * a.ks.row + h * a.ks.head, a.ks, m, p0);
+        raw[i].load(static_cast<const T*>(a.k) + a.ks.at(r) + h * a.ks.head, a.ks, m, p0);
     }
   }
   // The rotation is done twice, for the block's magnitude and for its codes:
@@ -534,7 +537,7 @@ struct VBlock {
         if (r < 0)
           raw[i][j].zero();
         else
-          load_run<T, Fast>(raw[i][j], static_cast<const T*>(a.v) + r * a.vs.row + h * a.vs.head + e * a.vs.elem, a.vs);
+          load_run<T, Fast>(raw[i][j], static_cast<const T*>(a.v) + a.vs.at(r) + h * a.vs.head + e * a.vs.elem, a.vs);
       }
   }
   __device__ __forceinline__ void put(const AppendArgs& a, const int* rows, uint8_t* block, uint8_t* scale,
@@ -622,7 +625,7 @@ __device__ __forceinline__ void one_k8(const AppendArgs& a, int64_t r, int t, ui
     int was = 0;
     if (live) {
       was = *scale;
-      raw.load(static_cast<const T*>(a.k) + r * a.ks.row + h * a.ks.head, a.ks, m, p0);
+      raw.load(static_cast<const T*>(a.k) + a.ks.at(r) + h * a.ks.head, a.ks, m, p0);
     }
     if (!filled) {
       __syncwarp();
@@ -663,7 +666,7 @@ __device__ __forceinline__ void one_v8(const AppendArgs& a, int64_t r, int t, ui
       was[i] = 0;
       if (h < a.H && l < D / 8) {
         was[i] = scales[h];
-        load_run<T, Fast>(raw[i], static_cast<const T*>(a.v) + r * a.vs.row + h * a.vs.head + l * 8 * a.vs.elem, a.vs);
+        load_run<T, Fast>(raw[i], static_cast<const T*>(a.v) + a.vs.at(r) + h * a.vs.head + l * 8 * a.vs.elem, a.vs);
         old[i] = *reinterpret_cast<const uint4*>(blocks + (int64_t)h * kTok * D + v8_off(t & ~1, l * 8, D));
       }
     }
@@ -843,22 +846,22 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, PoolGeom
       const int64_t r0 = query_rows(a, &live);
       for (; live; live &= live - 1) {
         const int64_t r = r0 + __ffs(live) - 1;
-        turn_row_any<T, T>(a.rot, r, a.Hq, a.dqk, static_cast<const T*>(a.q) + r * a.qs.row, a.qs,
-                           static_cast<T*>(a.q_out) + r * a.qo.row, a.qo, cs[warp * kQueryRows]);
+        turn_row_any<T, T>(a.rot, r, a.Hq, a.dqk, static_cast<const T*>(a.q) + a.qs.at(r), a.qs,
+                           static_cast<T*>(a.q_out) + a.qo.at(r), a.qo, cs[warp * kQueryRows]);
       }
     }
     return;
   }
   const int count = *a.plan.count + 1;
-  const Strides ks{0, (int64_t)kTok * g.dqk, 1};
+  const Strides ks{0, 0, (int64_t)kTok * g.dqk, 1};
   const int64_t step = (int64_t)a.page_blocks * kWarps;
   for (int64_t u = (int64_t)blockIdx.x * kWarps + warp; u < (int64_t)count * kTok; u += step) {
     const int at = a.plan.list[u / kTok];
     const int r = a.plan.rows[(size_t)at * kTok + u % kTok];
     const int64_t slot = (int64_t)a.plan.keys[at] * kTok + u % kTok;
     if (r < 0 || slot < 0 || slot >= g.num_slots) continue;  // the latter: a plan of another pool
-    const T* k = static_cast<const T*>(a.k) + r * a.ks.row;
-    const T* v = static_cast<const T*>(a.v) + r * a.vs.row;
+    const T* k = static_cast<const T*>(a.k) + a.ks.at(r);
+    const T* v = static_cast<const T*>(a.v) + a.vs.at(r);
     TP *ko = pool + g.k_off(slot, layer, 0), *vo = pool + g.v_off(slot, layer, 0);
     if constexpr (D > 0) {
       const int runs = g.dv / 8;
@@ -883,10 +886,10 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, PoolGeom
 
 // Strides of a source, and whether its rows are contiguous and 16-byte aligned.
 template <typename T>
-bool take_strides(const int64_t (&s)[3], const void* base, Strides* out) {
-  *out = Strides{s[0], s[1], s[2]};
+bool take_strides(const int64_t (&s)[3], const void* base, int64_t tile, Strides* out) {
+  *out = Strides{tile ? tile : 16 * s[0], s[0], s[1], s[2]};
   constexpr int64_t e = 16 / sizeof(T);
-  return s[2] == 1 && s[0] % e == 0 && s[1] % e == 0 && (reinterpret_cast<uintptr_t>(base) & 15) == 0;
+  return s[2] == 1 && out->tile % e == 0 && s[0] % e == 0 && s[1] % e == 0 && (reinterpret_cast<uintptr_t>(base) & 15) == 0;
 }
 
 template <typename T, int DQK, int DV>
@@ -912,7 +915,7 @@ cudaError_t launch_append_full(dim3 grid, const AppendArgs& a, const PoolGeom& g
 
 template <typename T>
 imba_status_t launch_append(const imba_cache_desc& c, const imba_pool_desc& pool, const imba_append_desc& d,
-                            void* plan, cudaStream_t s) {
+                            void* plan, cudaStream_t s, int64_t k_tile, int64_t v_tile) {
   AppendArgs a;
   a.plan = plan_view(plan, d.num_rows);
   a.n = d.num_rows;
@@ -922,10 +925,10 @@ imba_status_t launch_append(const imba_cache_desc& c, const imba_pool_desc& pool
   a.dv = c.linear_dim;
   a.k = d.k, a.v = d.v, a.q = d.q, a.q_out = d.q_out;
   bool fast = d.rotary.rot_dim % 16 == 0;
-  fast &= take_strides<T>(d.k_stride, d.k, &a.ks);
-  fast &= take_strides<T>(d.v_stride, d.v, &a.vs);
-  const bool q_fast = take_strides<T>(d.q_stride, d.q, &a.qs);
-  const bool o_fast = take_strides<T>(d.q_out_stride, d.q_out, &a.qo);
+  fast &= take_strides<T>(d.k_stride, d.k, k_tile, &a.ks);
+  fast &= take_strides<T>(d.v_stride, d.v, v_tile, &a.vs);
+  const bool q_fast = take_strides<T>(d.q_stride, d.q, 0, &a.qs);
+  const bool o_fast = take_strides<T>(d.q_out_stride, d.q_out, 0, &a.qo);
   fast &= !d.q || (q_fast && o_fast);
   a.rot = d.rotary;
   a.slots = d.slots;

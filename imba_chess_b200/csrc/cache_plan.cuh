@@ -39,8 +39,13 @@ inline PlanView plan_view(void* plan, int32_t n) {
   return v;
 }
 
+// k_tile, v_tile: elements from rows 16 i to rows 16 (i + 1) of k and v, 0
+// when rows are evenly apart.
 template <typename T>
 imba_status_t launch_append(const imba_cache_desc& c, const imba_pool_desc& pool, const imba_append_desc& d,
-                            void* plan, cudaStream_t s);
+                            void* plan, cudaStream_t s, int64_t k_tile = 0, int64_t v_tile = 0);
+// The plan of `slots` in `plan` (imba_append_plan_bytes(num_rows) of device memory).
+cudaError_t launch_append_plan(int64_t num_slots, int32_t num_rows, const int32_t* slots, void* plan, int32_t* status,
+                               cudaStream_t s);
 
 }  // namespace imba

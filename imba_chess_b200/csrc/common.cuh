@@ -109,6 +109,10 @@ struct imba_model {
   bool simt_gemm = false;
   bool simt_attn = false;
   bool simt_board = false;
+  bool cache8 = false;  // the KV pool is in 8 bits (IMBA_FLAG_CACHE_E4M3)
+  imba_cache_desc cache() const {
+    return imba_cache_desc{d.num_layers, d.num_heads, d.attention_dim, d.linear_dim, cache8 ? IMBA_DTYPE_E4M3 : d.dtype};
+  }
   // bf16 models with the tensor-core board encoder: [d, 192] bf16 split copy
   // of the board projection (device memory owned by the handle), or null.
   void* board_proj3 = nullptr;
@@ -150,6 +154,13 @@ struct Workspace {
   int* counters;   // [kNumCounters] work-queue counters, zeroed at the start of every step
   int* recs;       // [2 R][kAttnRecInts] bf16 models: resolved attention work items
   float2* ml;      // [R, H]      bf16 models: (max, sum) of each row's pages-only attention pass
+  // pools in 8 bits: the layer's new keys and values, laid out like a pool's
+  // pages of one layer (row r in slot r), their slots 0, 1, .. and the plans
+  void* kv;
+  int* kv_slots;
+  void* append_plan;
+  size_t append_bytes;
+  void* attend_plan;
   size_t bytes;
 };
 

@@ -18,6 +18,11 @@ staging and keeps every prefix and node resident in a persistent pool.
 
 Every call runs the CUDA library; there is no CPU path.  Output logits and
 value logits are fp32; returned k/v are in the model dtype.
+
+With ``kv_dtype=torch.float8_e4m3fn`` the model's pools hold keys and values
+in 8 bits (``kvpool``), half of bf16: its steps round each block of 16 tokens
+and head to e4m3 with a power-of-two scale and attend over the codes
+(``paged``'s operators).  Weights and activations stay in ``dtype``.
 """
 
 from __future__ import annotations
@@ -29,7 +34,7 @@ from typing import Any, Mapping
 import numpy as np
 import torch
 
-from . import _native
+from . import _native, paged
 from .kvpool import PAGE, KVPool
 from .plan import DeviceStep, StepBuffers, StepPlan, piece_ids_from_tokens, side_ids_from_tokens
 from .weights import PackedWeights
@@ -70,7 +75,8 @@ class B200HSTUChessModel:
     training = False
 
     def __init__(self, state_dict: Mapping[str, Any], *, dtype: torch.dtype = torch.bfloat16,
-                 device: torch.device | str = "cuda", simt: tuple[str, ...] = ()) -> None:
+                 device: torch.device | str = "cuda", simt: tuple[str, ...] = (),
+                 kv_dtype: torch.dtype | None = None) -> None:
         """``simt`` is a test hook for bf16 models: component names ("gemm",
         "attn", "board") whose fp32-accumulating SIMT kernels replace the
         tensor-core ones, so tests can compare the two on identical inputs."""
@@ -80,6 +86,9 @@ class B200HSTUChessModel:
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.dtype = dtype
+        self.kv_dtype = kv_dtype or dtype
+        if self.kv_dtype not in (dtype, torch.float8_e4m3fn):
+            raise ValueError(f"kv_dtype must be the model's dtype ({dtype}) or torch.float8_e4m3fn, got {kv_dtype}")
         with torch.cuda.device(self.device):
             self.weights = PackedWeights(state_dict, dtype=dtype, device=self.device)
         d = self.weights.dims
@@ -104,6 +113,8 @@ class B200HSTUChessModel:
             if name not in _native.SIMT_FLAGS:
                 raise ValueError(f"unknown SIMT component {name!r}: use {sorted(_native.SIMT_FLAGS)}")
             flags |= _native.SIMT_FLAGS[name]
+        if self.kv_dtype == torch.float8_e4m3fn:
+            flags |= _native.FLAG_CACHE_E4M3
         self.weights.desc.flags = flags
         handle = ctypes.c_void_p()
         _native.check(self._lib.imba_model_create(ctypes.byref(self.weights.desc), ctypes.byref(handle)),
@@ -114,22 +125,24 @@ class B200HSTUChessModel:
 
     # ------------------------------------------------------------------
     @classmethod
-    def from_reference(cls, model, *, dtype: torch.dtype | None = None, device=None) -> "B200HSTUChessModel":
+    def from_reference(cls, model, *, dtype: torch.dtype | None = None, device=None,
+                       kv_dtype: torch.dtype | None = None) -> "B200HSTUChessModel":
         """Build from a reference ``HSTUChessModel`` instance (its state_dict)."""
         sd = model.state_dict()
         dev = device if device is not None else "cuda"
-        return cls(sd, dtype=dtype or torch.bfloat16, device=dev)
+        return cls(sd, dtype=dtype or torch.bfloat16, device=dev, kv_dtype=kv_dtype)
 
     @classmethod
     def from_checkpoint(cls, path, *, dtype: torch.dtype = torch.bfloat16, device=None,
-                        require_value_head: bool = False) -> "B200HSTUChessModel":
+                        require_value_head: bool = False,
+                        kv_dtype: torch.dtype | None = None) -> "B200HSTUChessModel":
         """Load a reference checkpoint file (plain or Ignite state dict) with
         the reference loader's key normalisation, value-head guard and strict
         key check (``weights.load_checkpoint_state_dict``)."""
         from .weights import load_checkpoint_state_dict
 
         sd = load_checkpoint_state_dict(path, require_value_head=require_value_head)
-        return cls(sd, dtype=dtype, device=device if device is not None else "cuda")
+        return cls(sd, dtype=dtype, device=device if device is not None else "cuda", kv_dtype=kv_dtype)
 
     def eval(self) -> "B200HSTUChessModel":
         return self
@@ -146,7 +159,7 @@ class B200HSTUChessModel:
     def new_pool(self, num_pages: int) -> KVPool:
         d = self.dims
         return KVPool(num_layers=d.num_layers, num_heads=d.num_heads, attention_dim=d.attention_dim,
-                      linear_dim=d.linear_dim, num_pages=num_pages, dtype=self.dtype, device=self.device)
+                      linear_dim=d.linear_dim, num_pages=num_pages, dtype=self.kv_dtype, device=self.device)
 
     def workspace(self, rows: int) -> torch.Tensor:
         need = int(self._lib.imba_step_workspace_bytes(self._handle, int(rows)))
@@ -160,6 +173,7 @@ class B200HSTUChessModel:
         """Enqueue one step on ``stream`` (default: torch's current stream)."""
         desc = dstep.desc
         rows = desc.num_rows
+        self._check_pool(pool)
 
         def ptr(t):
             return None if t is None else t.data_ptr()
@@ -173,6 +187,9 @@ class B200HSTUChessModel:
         desc.status = ptr(status if status is not None else self._status)
         ws = self.workspace(rows)
         s = stream if stream is not None else torch.cuda.current_stream(self.device)
+        if pool._fresh:
+            with torch.cuda.stream(s):
+                pool.begin_pages()
         with torch.cuda.device(self.device):
             code = self._lib.imba_step(self._handle, ctypes.byref(desc), ctypes.byref(pool.desc), ws.data_ptr(),
                                        ws.numel(), s.cuda_stream)
@@ -185,8 +202,20 @@ class B200HSTUChessModel:
             st.zero_()
             raise _native.ImbaError(code, "device-side check")
 
+    def _check_pool(self, pool: KVPool) -> None:
+        """A pool of another type or shape would be read as if it were one of this model's."""
+        d = self.dims
+        if (pool.dtype != self.kv_dtype or pool.num_layers != d.num_layers or pool.num_heads != d.num_heads
+                or pool.attention_dim != d.attention_dim or pool.linear_dim != d.linear_dim):
+            raise ValueError(f"the pool ({pool.dtype}, {pool.num_layers} layers, {pool.num_heads} heads of "
+                             f"{pool.attention_dim} / {pool.linear_dim}) is not one of this model's (new_pool)")
+
     def kv_scatter(self, pool: KVPool, layer: int, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         n = int(slots.numel())
+        self._check_pool(pool)
+        if pool.scales is not None:
+            paged.kv_append(pool, layer, paged.AppendPlan(pool, slots.reshape(-1), status=self._status), k, v)
+            return
         s = torch.cuda.current_stream(self.device)
         with torch.cuda.device(self.device):
             code = self._lib.imba_kv_scatter(self._handle, ctypes.byref(pool.desc), layer, n, slots.data_ptr(),
@@ -195,6 +224,7 @@ class B200HSTUChessModel:
 
     def kv_gather(self, pool: KVPool, layer: int, slots: torch.Tensor):
         n = int(slots.numel())
+        self._check_pool(pool)
         d = self.dims
         k = torch.empty((n, d.num_heads, d.attention_dim), dtype=self.dtype, device=self.device)
         v = torch.empty((n, d.num_heads, d.linear_dim), dtype=self.dtype, device=self.device)
@@ -390,6 +420,8 @@ class B200HSTUChessModel:
         pool = getattr(self, "_scratch", None)
         if pool is None or pool.num_pages < num_pages:
             pool = self._scratch = self.new_pool(max(num_pages, int(num_pages * 1.25), 64))
+        if pool.scales is not None:
+            pool.scales.zero_()  # every call starts on empty blocks
         return pool
 
     def _scatter_dense(self, pool: KVPool, layer: int, n: int, slots, ia, ib, k: torch.Tensor,
@@ -400,6 +432,11 @@ class B200HSTUChessModel:
             k = k.to(device=self.device, dtype=self.dtype)
         if v.device != self.device or v.dtype != self.dtype:
             v = v.to(device=self.device, dtype=self.dtype)
+        if pool.scales is not None:
+            a, b = ia.long(), ib.long()
+            plan = paged.AppendPlan(pool, slots, status=self._status)
+            paged.kv_append(pool, layer, plan, k[a, :, b], v[a, :, b])
+            return
         # [A, H, B, d] tensors: strides in the order (a, b, head, dim)
         sk = (ctypes.c_int64 * 4)(k.stride(0), k.stride(2), k.stride(1), k.stride(3))
         sv = (ctypes.c_int64 * 4)(v.stride(0), v.stride(2), v.stride(1), v.stride(3))

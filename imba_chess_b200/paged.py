@@ -144,10 +144,16 @@ class Rotary:
 class AppendPlan:
     """A step's rows by the pages they go to: row r's token is stored in slot
     ``slots[r]`` (page * 16 + offset; -1: a padding row).  Of rows with the
-    same slot the last one is stored."""
+    same slot the last one is stored.  ``status`` (int32 ``[1]``) is the word
+    that errors go to, the pool's by default."""
 
-    def __init__(self, pool: KVPool, slots) -> None:
-        _, desc, status, _ = _cache(pool)
+    def __init__(self, pool: KVPool, slots, *, status: torch.Tensor | None = None) -> None:
+        _, desc, pool_status, _ = _cache(pool)
+        if status is None:
+            status = pool_status
+        else:
+            _rows(status, pool, "status", (1,), torch.int32)
+        self._status = status
         self.pool = pool
         self.slots = _ints(slots, pool, "slots")
         if self.slots.dim() != 1:

@@ -76,11 +76,13 @@ class ActorInferenceServer:
 
     def __init__(self, *, model, device: torch.device | str, dtype: torch.dtype, require_value_head: bool = True,
                  profile_sync: bool = False, kv_pool_pages: int | None = None,
-                 kv_pool_bytes: int | None = None) -> None:
+                 kv_pool_bytes: int | None = None, kv_dtype: torch.dtype | None = None) -> None:
         device = torch.device(device)
         if not isinstance(model, B200HSTUChessModel):
             model_dtype = torch.float32 if dtype == torch.float32 else torch.bfloat16
-            model = B200HSTUChessModel.from_reference(model, dtype=model_dtype, device=device)
+            model = B200HSTUChessModel.from_reference(model, dtype=model_dtype, device=device, kv_dtype=kv_dtype)
+        elif kv_dtype not in (None, model.kv_dtype):
+            raise ValueError(f"the model keeps its KV in {model.kv_dtype}, not in {kv_dtype}")
         if require_value_head and getattr(model, "value_head", None) is None:
             raise ValueError(
                 "ActorInferenceServer(require_value_head=True) requires a model with an enabled value head: "
@@ -120,8 +122,9 @@ class ActorInferenceServer:
 
     def _page_bytes(self) -> int:
         d = self._model.dims
-        esize = 2 if self._model.dtype == torch.bfloat16 else 4
-        return d.num_layers * d.num_heads * PAGE * (d.attention_dim + d.linear_dim) * esize
+        per_head = PAGE * (d.attention_dim + d.linear_dim) * self._model.kv_dtype.itemsize
+        scales = 2 if self._model.kv_dtype == torch.float8_e4m3fn else 0
+        return d.num_layers * d.num_heads * (per_head + scales)
 
     # ------------------------------------------------------------------
     def register_root(self, worker_id: int, turn_id: int, batch_arrays: dict, legal_vocab_ids: list[int]):

@@ -58,10 +58,17 @@ typedef int32_t imba_status_t;
 
 /* imba_model_desc.flags: test hooks that replace one tensor-core component of
  * a bf16 handle by its fp32-accumulating SIMT kernel, so a test can compare
- * the two on identical inputs.  Production handles pass 0. */
+ * the two on identical inputs.  Production handles pass none of them. */
 #define IMBA_FLAG_SIMT_GEMM 1   /* projections, heads: SIMT GEMMs                 */
 #define IMBA_FLAG_SIMT_ATTN 2   /* attention: SIMT kernel + separate gate pass    */
 #define IMBA_FLAG_SIMT_BOARD 4  /* board encoder + content: fp32 SIMT kernel      */
+/* Not a test hook: the handle's KV pool is in 8 bits ("Cache operators"
+ * below; its geometry is imba_cache_desc {num_layers, num_heads,
+ * attention_dim, linear_dim, IMBA_DTYPE_E4M3}).  Steps append to it and attend
+ * over it with the cache operators' kernels; imba_kv_gather reads it, and
+ * imba_kv_scatter / _indexed return IMBA_ERR_UNSUPPORTED (imba_kv_append
+ * writes it).  Head dims as for such a pool, else IMBA_ERR_UNSUPPORTED. */
+#define IMBA_FLAG_CACHE_E4M3 8
 
 #define IMBA_MAX_LAYERS 32
 #define IMBA_PAGE_TOKENS 16     /* tokens per KV page                              */
@@ -85,7 +92,7 @@ typedef struct imba_model_desc {
   int32_t fullmove_vocab;
   int32_t has_value_head;
   int32_t dtype;            /* IMBA_DTYPE_*                        */
-  int32_t flags;            /* IMBA_FLAG_* (0 for normal use)      */
+  int32_t flags;            /* IMBA_FLAG_*                         */
 
   /* content embedding (hstu_model.py:209-228, :275-335) */
   const float* piece_square;   /* [832, 64]                                */
