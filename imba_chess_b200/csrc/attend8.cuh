@@ -13,6 +13,7 @@ namespace imba {
 // is an item and a key / value head.
 constexpr int kTileRows = 8;
 constexpr int kUnitWarps = 8;  // warps of a CTA
+constexpr int kTileGroups = 16;  // rt of the tcgen05 kernel's tiles of 128 rows
 
 struct AttendRow {  // one flattened row of a tile
   int row;          // -1: none
@@ -33,7 +34,7 @@ struct AttendItem {
 
 struct AttendShape {
   int share;        // query heads per key / value head
-  int rt;           // 8-row groups of a tile: 1 or 2
+  int rt;           // 8-row groups of a tile: 1, 2 or kTileGroups
   int warps;        // warps that share a unit: 1 or kUnitWarps
   int tile_rows;    // kTileRows * rt
   int max_tiles;
@@ -50,7 +51,7 @@ struct AttendPlan {
   int4* tiles;           // {segment, first flattened row, rows, visible pages}
   AttendItem* items;
   AttendRow* rows;       // [max_tiles][tile_rows]
-  int* done;             // [max_tiles][H] items of a split tile that have finished
+  int* done;             // [max_tiles][H][8] items of a split tile (or of a part of its rows) that have finished
   float2* ml;            // [max_parts][H][tile_rows] running maximum and sum
   float* o;              // [max_parts][H][tile_rows][d_v]
   size_t bytes;
@@ -74,6 +75,7 @@ struct AttendArgs {
 
 template <typename T>
 cudaError_t launch_attend8(const imba_cache_desc& c, const AttendArgs& a, cudaStream_t s);
+cudaError_t launch_attend8_tile(const imba_cache_desc& c, const AttendArgs& a, cudaStream_t s);
 cudaError_t launch_attend_plan(const imba_cache_desc& c, const imba_attend_desc& r, const AttendShape& sh,
                                const AttendPlan& p, cudaStream_t s);
 imba_status_t validate_cache(const imba_cache_desc* c);

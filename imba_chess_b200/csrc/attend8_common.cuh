@@ -1,0 +1,106 @@
+// Attention over a paged pool in 8 bits: numerics and the join of split
+// sequences, shared by the mma.sync kernel (few rows a segment) and the
+// tcgen05 kernel (many).
+#pragma once
+
+#include "attend8.cuh"
+
+namespace imba {
+
+namespace {
+
+constexpr float kShift = 5.f;
+constexpr float kSlack = 4.f;
+constexpr int kVWindow = 6;  // 2^(kShift + kSlack + kVWindow) = 2^15 is finite in f16
+
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_h2(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+
+// Scores are kept in log2 without a bias (the factor log2 e joins the
+// query's), with one as natural logarithms, where the bias is added as it is;
+// `lg` takes them to log2.  A bias below kFar that is not -inf counts as
+// kFar, a power of two, whose product with lg is exact: a row whose every key
+// carries the type's lowest value still weighs its keys by nothing else.
+constexpr float kFar = -1.2676506002282294e30f;  // -2^100
+__device__ __forceinline__ float take_bias(float b) { return b == -INFINITY ? b : fmaxf(b, kFar); }
+
+// exp of a difference of running maxima; 0 for a part that has seen nothing.
+__device__ __forceinline__ float weight_of(float a, float b, float lg) {
+  return a == -INFINITY ? 0.f : exp2_approx((a - b) * lg);
+}
+
+// Four consecutive elements of a row as floats.
+template <typename T>
+__device__ __forceinline__ void q_load4(const T* p, bool vec, float (&x)[4]) {
+  if (vec) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 f = *reinterpret_cast<const float4*>(p);
+      x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+      const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+      x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = to_f(p[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void out_store4(T* p, bool vec, const float (&x)[4]) {
+  if (vec) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+      __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+      *reinterpret_cast<uint2*>(p) =
+          make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = from_f<T>(x[i]);
+  }
+}
+
+// Rows r0 .. r0 + n - 1 of a split tile joined over its items, by `nthr`
+// threads from tid on.
+template <typename T, int DV>
+__device__ __forceinline__ void join_items(const AttendArgs& a, const AttendItem& it, int head, float lg, int r0, int n,
+                                           int tid, int nthr) {
+  const int H = a.cache.H;
+  const size_t first = (size_t)(it.part - it.index) * H + head;
+  const int tile_rows = a.shape.tile_rows;
+  const AttendRow* rows = a.plan.rows + (size_t)it.tile * tile_rows;
+  const bool vec = a.call.out_stride[0] % 4 == 0 && a.call.out_stride[1] % 4 == 0 &&
+                   (reinterpret_cast<uintptr_t>(a.call.out) & (4 * sizeof(T) - 1)) == 0;
+  for (int i = tid; i < n * (DV / 4); i += nthr) {
+    const int r = r0 + i / (DV / 4), e = i % (DV / 4) * 4;
+    const AttendRow row = rows[r];
+    if (row.row < 0) continue;
+    float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < it.splits; ++s)
+      m = fmaxf(m, __ldcg(a.plan.ml + (first + (size_t)s * H) * tile_rows + r).x);
+    for (int s = 0; s < it.splits; ++s) {
+      const size_t at = (first + (size_t)s * H) * tile_rows + r;
+      const float2 ml = __ldcg(a.plan.ml + at);
+      const float w = weight_of(ml.x, m, lg);
+      const float4 o = __ldcg(reinterpret_cast<const float4*>(a.plan.o + at * DV + e));
+      l += w * ml.y;
+      x[0] += w * o.x, x[1] += w * o.y, x[2] += w * o.z, x[3] += w * o.w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] *= inv;
+    out_store4(static_cast<T*>(a.call.out) + row.row * a.call.out_stride[0] +
+                   (int64_t)(head * a.shape.share + row.head) * a.call.out_stride[1] + e,
+               vec, x);
+  }
+}
+
+}  // namespace
+
+}  // namespace imba

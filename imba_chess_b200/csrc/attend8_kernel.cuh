@@ -36,15 +36,11 @@
 // rescaled, a power of two).  Sums, maxima and weights are fp32.
 #pragma once
 
-#include "attend8.cuh"
+#include "attend8_common.cuh"
 
 namespace imba {
 
 namespace {
-
-constexpr float kShift = 5.f;
-constexpr float kSlack = 4.f;
-constexpr int kVWindow = 6;  // 2^(kShift + kSlack + kVWindow) = 2^15 is finite in f16
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -59,12 +55,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-
-__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack_h2(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
 
 // (lo, hi) as f16 pairs: the rounded values, and with NP == 2 what is left.
 template <int NP>
@@ -116,53 +106,6 @@ __device__ __forceinline__ float keys_sum(float x) {
   return x;
 }
 
-// Scores are kept in log2 without a bias (the factor log2 e joins the
-// query's), with one as natural logarithms, where the bias is added as it is;
-// `lg` takes them to log2.  A bias below kFar that is not -inf counts as
-// kFar, a power of two, whose product with lg is exact: a row whose every key
-// carries the type's lowest value still weighs its keys by nothing else.
-constexpr float kFar = -1.2676506002282294e30f;  // -2^100
-__device__ __forceinline__ float take_bias(float b) { return b == -INFINITY ? b : fmaxf(b, kFar); }
-
-// exp of a difference of running maxima; 0 for a part that has seen nothing.
-__device__ __forceinline__ float weight_of(float a, float b, float lg) {
-  return a == -INFINITY ? 0.f : exp2_approx((a - b) * lg);
-}
-
-// Four consecutive elements of a row as floats.
-template <typename T>
-__device__ __forceinline__ void q_load4(const T* p, bool vec, float (&x)[4]) {
-  if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 f = *reinterpret_cast<const float4*>(p);
-      x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(p);
-      const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
-      const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
-      x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = to_f(p[i]);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void out_store4(T* p, bool vec, const float (&x)[4]) {
-  if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-    } else {
-      __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
-      *reinterpret_cast<uint2*>(p) =
-          make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = from_f<T>(x[i]);
-  }
-}
-
 // Sizes that follow from the head dimensions.  RT: groups of eight rows.
 template <int DQK, int DV, int RT>
 struct Dims {
@@ -173,40 +116,6 @@ struct Dims {
   static constexpr int STAGE = IMBA_PAGE_TOKENS * (DQK + DV);  // a warp's page
   static constexpr int MERGE = kUnitWarps * ROWS * (DV * 4 + 8) + 16;
 };
-
-// Tile rows joined over the items of a split tile; `nthr` threads from tid on.
-template <typename T, int DQK, int DV, int RT>
-__device__ __forceinline__ void join_items(const AttendArgs& a, const AttendItem& it, int head, float lg, int tid,
-                                           int nthr) {
-  using D = Dims<DQK, DV, RT>;
-  const int H = a.cache.H;
-  const size_t first = (size_t)(it.part - it.index) * H + head;
-  const AttendRow* rows = a.plan.rows + (size_t)it.tile * D::ROWS;
-  const bool vec = a.call.out_stride[0] % 4 == 0 && a.call.out_stride[1] % 4 == 0 &&
-                   (reinterpret_cast<uintptr_t>(a.call.out) & (4 * sizeof(T) - 1)) == 0;
-  for (int i = tid; i < D::ROWS * (DV / 4); i += nthr) {
-    const int r = i / (DV / 4), e = i % (DV / 4) * 4;
-    const AttendRow row = rows[r];
-    if (row.row < 0) continue;
-    float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < it.splits; ++s)
-      m = fmaxf(m, __ldcg(a.plan.ml + (first + (size_t)s * H) * D::ROWS + r).x);
-    for (int s = 0; s < it.splits; ++s) {
-      const size_t at = (first + (size_t)s * H) * D::ROWS + r;
-      const float2 ml = __ldcg(a.plan.ml + at);
-      const float w = weight_of(ml.x, m, lg);
-      const float4 o = __ldcg(reinterpret_cast<const float4*>(a.plan.o + at * DV + e));
-      l += w * ml.y;
-      x[0] += w * o.x, x[1] += w * o.y, x[2] += w * o.z, x[3] += w * o.w;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] *= inv;
-    out_store4(static_cast<T*>(a.call.out) + row.row * a.call.out_stride[0] +
-                   (int64_t)(head * a.shape.share + row.head) * a.call.out_stride[1] + e,
-               vec, x);
-  }
-}
 
 // A warp's rows and what they have summed up: lane (g, t) = (lane / 4, lane %
 // 4) holds rows 8 i + 2 t + r, i < RT, r < 2, of scores and weights for keys g
@@ -307,12 +216,16 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
   const int sub = NW == 1 ? 0 : warp;
   const int H = a.cache.H;
   const uint32_t unit = NW == 1 ? blockIdx.x * kUnitWarps + warp : blockIdx.x;
-  const int item_id = (int)(unit / (uint32_t)H), head = (int)(unit % (uint32_t)H);
+  // (a plan with tiles of 128 rows: eight units of sixteen a tile)
+  const int subs = a.shape.tile_rows / D::ROWS, sub_tile = subs > 1 ? (int)(unit % (uint32_t)subs) : 0;
+  const uint32_t whole = subs > 1 ? unit / (uint32_t)subs : unit;
+  const int item_id = (int)(whole / (uint32_t)H), head = (int)(whole % (uint32_t)H);
   if (item_id >= a.shape.max_items) return;
   const int items = a.plan.head[0];
   const AttendItem it = a.plan.items[item_id];  // together with the count
   if (item_id >= items) return;
-  const int4* tile = reinterpret_cast<const int4*>(a.plan.rows + (size_t)it.tile * D::ROWS);
+  const int r0 = sub_tile * D::ROWS;
+  const int4* tile = reinterpret_cast<const int4*>(a.plan.rows + (size_t)it.tile * a.shape.tile_rows + r0);
 
   // This warp's pages: list entries sub, sub + NW, ... of the item, 32 at a
   // time in the lanes (id and the two scale bytes), the next 32 in flight.
@@ -704,7 +617,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
   auto dim = [&](int c, int q) { return c * 4 * D::VV + g * (D::VV / 2) + 4 * q; };
 
   if constexpr (NW == 1) {
-    const size_t part = ((size_t)max(it.part, 0) * H + head) * D::ROWS;
+    const size_t part = ((size_t)max(it.part, 0) * H + head) * a.shape.tile_rows + r0;
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -731,13 +644,13 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
     if (it.part >= 0) {
       __threadfence();
       __syncwarp();
-      int* done = a.plan.done + (size_t)it.tile * H + head;
+      int* done = a.plan.done + ((size_t)it.tile * H + head) * subs + sub_tile;
       int n = 0;
       if (lane == 0) n = atomicAdd(done, 1);
       if (__shfl_sync(0xffffffffu, n, 0) == it.splits - 1) {  // the others have finished
         __threadfence();
         if (lane == 0) *done = 0;
-        join_items<T, DQK, DV, RT>(a, it, head, st.lg, lane, 32);
+        join_items<T, DV>(a, it, head, st.lg, r0, D::ROWS, lane, 32);
       }
     }
   } else {
@@ -765,7 +678,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
           }
       }
     __syncthreads();
-    const size_t part = ((size_t)max(it.part, 0) * H + head) * D::ROWS;
+    const size_t part = ((size_t)max(it.part, 0) * H + head) * a.shape.tile_rows + r0;
     for (int i = threadIdx.x; i < D::ROWS * (DV / 4); i += kUnitWarps * 32) {
       const int tr = i / (DV / 4), e = i % (DV / 4) * 4;
       const int4 row = __ldg(tile + tr);
@@ -796,13 +709,13 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
     if (it.part >= 0) {
       __threadfence();
       __syncthreads();
-      int* done = a.plan.done + (size_t)it.tile * H + head;
+      int* done = a.plan.done + ((size_t)it.tile * H + head) * subs + sub_tile;
       if (threadIdx.x == 0) *flag = atomicAdd(done, 1) == it.splits - 1;
       __syncthreads();
       if (*flag) {
         __threadfence();
         if (threadIdx.x == 0) *done = 0;
-        join_items<T, DQK, DV, RT>(a, it, head, st.lg, threadIdx.x, kUnitWarps * 32);
+        join_items<T, DV>(a, it, head, st.lg, r0, D::ROWS, threadIdx.x, kUnitWarps * 32);
       }
     }
   }
@@ -819,7 +732,7 @@ cudaError_t launch_one(const AttendArgs& a, cudaStream_t s) {
   auto fn = attend8_kernel<T, DQK, DV, RT, NW, kStages, kCtas>;
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  const int64_t units = (int64_t)a.shape.max_items * a.cache.H;
+  const int64_t units = (int64_t)a.shape.max_items * a.cache.H * (a.shape.tile_rows / D::ROWS);
   const int64_t grid = NW == 1 ? (units + kUnitWarps - 1) / kUnitWarps : units;
   if (units > INT32_MAX) return cudaErrorInvalidValue;
   return launch_pdl(fn, dim3((unsigned)grid), dim3(kUnitWarps * 32), smem, s, a);
@@ -834,6 +747,7 @@ cudaError_t launch_rows(const AttendArgs& a, cudaStream_t s) {
 
 template <typename T>
 cudaError_t launch_attend8(const imba_cache_desc& c, const AttendArgs& a, cudaStream_t s) {
+  if (a.shape.rt == kTileGroups && sizeof(T) == 2) return launch_attend8_tile(c, a, s);
 #define IMBA_ATTEND8(DQK, DV)                                              \
   if (c.attention_dim == DQK && c.linear_dim == DV) {                      \
     if (a.shape.rt == 1) return launch_rows<T, DQK, DV, 1>(a, s);          \

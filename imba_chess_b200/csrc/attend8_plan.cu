@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kPlanThreads) attend_items_kernel(imba_attend_
     p.tiles[2 * t] = make_int4(lo, f0, nf, pages);
     p.tiles[2 * t + 1] = make_int4(off, first, count, vmin);
     mine += pages;
-    for (int h = 0; h < H; ++h) p.done[(size_t)t * H + h] = 0;
+    for (int h = 0; h < 8 * H; ++h) p.done[(size_t)t * 8 * H + h] = 0;
   }
   if (mine) atomicAdd(&all_pages, mine);
   __syncthreads();
@@ -196,6 +196,10 @@ __global__ void attend_rows_kernel(imba_attend_desc r, AttendShape sh, AttendPla
 
 namespace {
 
+// Rows a segment (with its shared heads) from which the tcgen05 kernel's tiles
+// of 128 are better than tiles of 16 by mma.sync.
+constexpr int64_t kTileFrom = 64;
+
 // The shape with tiles of 8 rt rows and `warps` warps a unit.
 AttendShape shape_of(const imba_cache_desc& c, const imba_attend_desc& r, int rt, int warps, int64_t most) {
   AttendShape sh;
@@ -207,8 +211,10 @@ AttendShape shape_of(const imba_cache_desc& c, const imba_attend_desc& r, int rt
   sh.max_tiles = (int)std::min<int64_t>(tiles, INT32_MAX);
   sh.warps = warps;
   sh.min_pages = warps == 1 ? 16 : 8;
-  // About four CTAs' worth of units for each that is resident.
-  sh.target = (int)std::min<int64_t>(most, std::max(1, 148 * 2 * 4 * (kUnitWarps / warps) / c.num_heads));
+  // About four CTAs' worth of units for each that is resident (two of the
+  // tcgen05 kernel's, whose parts are large).
+  const int waves = rt == kTileGroups ? 2 : 4;
+  sh.target = (int)std::min<int64_t>(most, std::max(1, 148 * 2 * waves * (kUnitWarps / warps) / c.num_heads));
   const int64_t by_len = (int64_t)sh.max_tiles * ((r.num_group_pages + sh.min_pages - 1) / sh.min_pages);
   const int64_t cut = std::min<int64_t>(by_len, sh.target);  // full-size items; each tile may add one smaller
   sh.max_items = (int)std::min<int64_t>(sh.max_tiles + cut, INT32_MAX / 4);
@@ -222,6 +228,8 @@ AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r, in
   const int64_t flat = (int64_t)r.num_rows * (r.num_q_heads / c.num_heads);
   // Rows of a tile by what a segment has on average.
   const int64_t per_seg = r.num_segs ? (flat + r.num_segs - 1) / r.num_segs : 0;
+  if (r.num_extra == 0 && c.attention_dim == c.linear_dim && c.attention_dim % 64 == 0 && per_seg >= kTileFrom)
+    return shape_of(c, r, kTileGroups, kUnitWarps, most);
   const int rt = per_seg <= 8 ? 1 : 2;
   // One warp per unit when there are enough units to fill the device and the
   // page lists are short on average; else the CTA's warps share a unit.
@@ -236,7 +244,7 @@ size_t attend_step_bytes(const imba_cache_desc& c, int32_t rows) {
   r.num_group_pages = INT32_MAX / IMBA_PAGE_TOKENS;
   r.num_q_heads = c.num_heads;
   size_t most = 0;
-  for (int rt = 1; rt <= 2; ++rt)
+  for (int rt : {1, 2, kTileGroups})
     for (int warps : {1, kUnitWarps})
       most = std::max(most, attend_plan_view(c, r, shape_of(c, r, rt, warps, attend_step_most(rows)), nullptr).bytes);
   return most;
@@ -256,7 +264,7 @@ AttendPlan attend_plan_view(const imba_cache_desc& c, const imba_attend_desc& r,
   p.tiles = static_cast<int4*>(take((size_t)sh.max_tiles * 2 * sizeof(int4)));
   p.items = static_cast<AttendItem*>(take((size_t)sh.max_items * sizeof(AttendItem)));
   p.rows = static_cast<AttendRow*>(take((size_t)sh.max_tiles * sh.tile_rows * sizeof(AttendRow)));
-  p.done = static_cast<int*>(take((size_t)sh.max_tiles * c.num_heads * sizeof(int)));
+  p.done = static_cast<int*>(take((size_t)sh.max_tiles * c.num_heads * 8 * sizeof(int)));
   p.ml = static_cast<float2*>(take((size_t)sh.max_parts * c.num_heads * sh.tile_rows * sizeof(float2)));
   p.o = static_cast<float*>(take((size_t)sh.max_parts * c.num_heads * sh.tile_rows * c.linear_dim * sizeof(float)));
   p.bytes = off;

@@ -510,6 +510,110 @@ def test_attention_reports_what_it_skips():
     run(row_extra_off=[0, 5, 1, 1], extra_slot=[1], extra_pos=[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("heads,share,d", [(2, 1, 64), (1, 5, 64), (1, 2, 128)])
+def test_attention_many_rows(heads, share, d, dtype):
+    """Segments of many rows (tiles of 128 on the tensor cores, or of fewer
+    rows by parts): causal parts and whole ones, some that see nothing, ends
+    inside a page, a block and a tile, a bias that ends inside."""
+    rng = np.random.default_rng(heads * 100 + share * 10 + d)
+    lens = [0, 1, 16, 63, 64, 65, 130, 300]
+    nrow = [70, 65, 64, 130, 80, 65, 130, 90]
+    pool = _pool(heads=heads, dqk=d, dv=d, pages=60, layers=2)
+    page_off, pages, _ = _fill(pool, rng, lens, layer=1)
+    row_off = np.r_[0, np.cumsum(nrow)]
+    vis = np.concatenate([[max(0, n - r + 1 + i) if n % 2 else n for i in range(r)] for n, r in zip(lens, nrow)])
+    pos = vis + rng.integers(0, 4, len(vis))
+    q = _rand(rng, (len(vis), heads * share, d), dtype, 0.3)
+    bias = torch.tensor(rng.standard_normal((heads * share, 201)), dtype=torch.float32, device=DEV)
+    plan = paged.AttentionPlan(pool, row_off=row_off, row_vis=vis, page_off=page_off, pages=pages,
+                               num_q_heads=heads * share, positions=pos)
+    for b, scale in ((None, None), (bias, -0.3)):
+        got = paged.paged_attention(pool, 1, plan, q, bias=b, scale=scale)
+        paged.check_status(pool)
+        _compare(got, _reference(pool, 1, q, scale or d**-0.5, row_off, vis, page_off, pages,
+                                 None if b is None else _f64(b), pos))
+        assert torch.equal(got, paged.paged_attention(pool, 1, plan, q, bias=b, scale=scale))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_many_rows_split(d):
+    """Few tiles over long lists: their parts are joined."""
+    rng = np.random.default_rng(d)
+    pool = _pool(heads=1, dqk=d, dv=d, pages=520)
+    n, rows = [5001, 3000], [70, 65]
+    page_off, pages, _ = _fill(pool, rng, n)
+    row_off = np.array([0, 70, 135])
+    vis = np.r_[5001 - 69 + np.arange(70), np.full(65, 3000)]
+    q = _rand(rng, (135, 2, d), torch.bfloat16, 0.3)
+    plan = paged.AttentionPlan(pool, row_off=row_off, row_vis=vis, page_off=page_off, pages=pages, num_q_heads=2)
+    for _ in range(3):
+        got = paged.paged_attention(pool, 0, plan, q)
+    paged.check_status(pool)
+    _compare(got, _reference(pool, 0, q, d**-0.5, row_off, vis, page_off, pages))
+    for x in (q.float(), q):  # the same plan for fp32 rows, and back
+        got = paged.paged_attention(pool, 0, plan, x)
+    _compare(got, _reference(pool, 0, q, d**-0.5, row_off, vis, page_off, pages))
+
+
+def test_attention_many_rows_scales_far_apart():
+    """V scales that differ within a block of 64 keys, by more than one
+    reference holds: rows that see the small ones alone keep their precision."""
+    rng = np.random.default_rng(43)
+    pool = _pool(heads=1, pages=20)
+    sizes = [1.0, 1e-6, 1e6, 1e-12, 3e4, 1e-3, 1e9, 1.0, 1e-9, 1e-9, 1e-9, 1e-9, 2.0, 1e-2]
+    page_off, pages, slots = _fill(pool, rng, [16 * len(sizes)], dtype=torch.float32)
+    pool.begin_pages(pages)
+    n = len(slots)
+    k = _rand(rng, (n, 1, 64), torch.float32, 0.5) * 0.05
+    v = _rand(rng, (n, 1, 64), torch.float32, 0.5) * torch.tensor(np.repeat(sizes, 16), dtype=torch.float32, device=DEV)[:, None, None]
+    paged.kv_append(pool, 0, paged.AppendPlan(pool, slots), k, v)
+    vis = np.r_[np.arange(0, 130), np.full(20, n), np.arange(150, 200)]
+    bias = np.zeros((1, 2 * n - 1))
+    bias[0, : n - 1 - 30] = -60.0  # keys more than 30 back count for little: late rows see small V's
+    bias = torch.tensor(bias, dtype=torch.float32, device=DEV)
+    q = _rand(rng, (len(vis), 1, 64), torch.bfloat16, 0.3)
+    row_off = np.array([0, len(vis)])
+    plan = paged.AttentionPlan(pool, row_off=row_off, row_vis=vis, page_off=page_off, pages=pages, num_q_heads=1, positions=vis)
+    for b in (None, bias):
+        got = paged.paged_attention(pool, 0, plan, q, bias=b)
+        paged.check_status(pool)
+        _compare(got, _reference(pool, 0, q, 0.125, row_off, vis, page_off, pages, None if b is None else _f64(b), vis))
+
+
+def test_attention_many_rows_other_cases():
+    """Not finite queries stay in their rows, strided rows, rows left alone
+    and bad pages, on tiles of 128 rows."""
+    rng = np.random.default_rng(47)
+    pool = _pool(heads=1, pages=16)
+    page_off, pages, _ = _fill(pool, rng, [100, 40])
+    row_off, vis = np.array([0, 70, 140]), np.r_[np.full(70, 100), np.arange(70) % 41, [5, 5]]
+    wide = _rand(rng, (142, 2, 67), torch.bfloat16, 0.3)
+    room = torch.full((142, 3, 67), 9.0, dtype=torch.bfloat16, device=DEV)
+    q, out = wide[..., 3:], room[:, 1:, 3:]
+    plan = paged.AttentionPlan(pool, row_off=row_off, row_vis=vis, page_off=page_off, pages=pages, num_q_heads=2)
+    paged.paged_attention(pool, 0, plan, q, out=out)
+    paged.check_status(pool)
+    _compare(out[:140], _reference(pool, 0, q[:140], 0.125, row_off, vis, page_off, pages))
+    good = paged.paged_attention(pool, 0, plan, q.contiguous())[:140]
+    assert torch.equal(out[:140], good)
+    assert (room[140:] == 9).all() and (room[:, 0] == 9).all() and (room[..., :3] == 9).all()
+    odd = q.contiguous()
+    odd[3, 1, 7], odd[5, 0, 0] = math.nan, math.inf
+    got = paged.paged_attention(pool, 0, plan, odd)[:140]
+    assert torch.isnan(got[3, 1]).all() and torch.isnan(got[5, 0]).all()
+    got[3, 1], got[5, 0] = good[3, 1], good[5, 0]
+    assert torch.equal(got, good)
+    for bad in (-1, 16, 2**31 - 1):
+        wrong = pages.copy()
+        wrong[1] = bad
+        plan = paged.AttentionPlan(pool, row_off=row_off, row_vis=vis, page_off=page_off, pages=wrong, num_q_heads=2)
+        got = paged.paged_attention(pool, 0, plan, q.contiguous())[:140]
+        with pytest.raises(_native.ImbaError):
+            paged.check_status(pool)
+        assert torch.isfinite(got).all() and torch.equal(got[70:], good[70:])
+
+
 def test_operators_together_under_a_graph():
     """Decode steps as a program runs them: a plan per step, append and
     attention for every layer, captured and replayed on another stream; the
