@@ -77,20 +77,37 @@ __device__ __forceinline__ void join_items(const AttendArgs& a, const AttendItem
   const AttendRow* rows = a.plan.rows + (size_t)it.tile * tile_rows;
   const bool vec = a.call.out_stride[0] % 4 == 0 && a.call.out_stride[1] % 4 == 0 &&
                    (reinterpret_cast<uintptr_t>(a.call.out) & (4 * sizeof(T) - 1)) == 0;
+  constexpr int kAhead = 4;  // parts in flight
   for (int i = tid; i < n * (DV / 4); i += nthr) {
     const int r = r0 + i / (DV / 4), e = i % (DV / 4) * 4;
     const AttendRow row = rows[r];
     if (row.row < 0) continue;
     float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < it.splits; ++s)
-      m = fmaxf(m, __ldcg(a.plan.ml + (first + (size_t)s * H) * tile_rows + r).x);
-    for (int s = 0; s < it.splits; ++s) {
-      const size_t at = (first + (size_t)s * H) * tile_rows + r;
-      const float2 ml = __ldcg(a.plan.ml + at);
-      const float w = weight_of(ml.x, m, lg);
-      const float4 o = __ldcg(reinterpret_cast<const float4*>(a.plan.o + at * DV + e));
-      l += w * ml.y;
-      x[0] += w * o.x, x[1] += w * o.y, x[2] += w * o.z, x[3] += w * o.w;
+    for (int s0 = 0; s0 < it.splits; s0 += kAhead) {
+      float2 ml[kAhead];
+      float4 o[kAhead];
+      float now = m;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        ml[j] = make_float2(-INFINITY, 0.f);
+        if (s0 + j >= it.splits) continue;
+        const size_t at = (first + (size_t)(s0 + j) * H) * tile_rows + r;
+        ml[j] = __ldcg(a.plan.ml + at);
+        o[j] = __ldcg(reinterpret_cast<const float4*>(a.plan.o + at * DV + e));
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) now = fmaxf(now, ml[j].x);
+      const float was = weight_of(m, now, lg);
+      l *= was;
+      x[0] *= was, x[1] *= was, x[2] *= was, x[3] *= was;
+      m = now;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (s0 + j >= it.splits) continue;
+        const float w = weight_of(ml[j].x, m, lg);
+        l += w * ml[j].y;
+        x[0] += w * o[j].x, x[1] += w * o[j].y, x[2] += w * o[j].z, x[3] += w * o[j].w;
+      }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll

@@ -8,10 +8,13 @@
 // e4m3 is exact in f16, so four warps turn the pages' codes into f16 tiles in
 // shared memory (K by rows of dimensions, V by rows of a token's dimensions,
 // an MN-major operand; both with the 128-byte swizzle), one block ahead of the
-// products; four warps are the tile's rows, one thread a row: they read S from
-// TMEM, weigh it and write P; a lane of the last page warp issues the
-// products, S of a block before P V of the one before it, which is what its
-// own next block waits for.  Scales stay out of the products: K's
+// products; eight warps are the tile's rows, two threads a row, each with half
+// of a block's keys (one thread a row and all 64 keys left the SM waiting for
+// its instructions: 215 us against 145 for 4 x 512 rows of 16 heads over 2k to
+// 8k tokens): they read S from TMEM, agree on the row's maximum, weigh and
+// write P; a lane of the last page warp issues the
+// products: P V of a block, S of the block after next (whose tiles are ready:
+// three stages), and then turns its page of the block that P V makes room for.  Scales stay out of the products: K's
 // multiplies a page's scores, V's is in its weights' exponent.
 //
 // What bounds it: the exponentials and the few instructions a score takes
@@ -33,8 +36,11 @@ namespace {
 constexpr int kRows = 128;
 constexpr int kKeys = 64;
 constexpr int kPages = kKeys / IMBA_PAGE_TOKENS;
-constexpr int kTileThreads = 256;  // warps 0-3: rows; 4-7: pages, and 7 the products
+constexpr int kTileThreads = 384;  // warps 0-7: rows; 8-11: pages, and 11 the products
+constexpr int kRowWarps = 8;
+constexpr int kHalf = kKeys / 2;   // keys of a row thread
 constexpr uint32_t kCols = 256;    // TMEM columns: S at 0 and 64, O from 128
+constexpr int kStages = 3;         // blocks of K and V
 constexpr int kSpread = 12;        // with kVWindow on both sides
 constexpr uint32_t kPanel = 128;   // bytes of a swizzled row: 64 f16
 constexpr uint32_t kKvPanel = kKeys * kPanel, kRowPanel = kRows * kPanel;
@@ -49,14 +55,44 @@ struct TileMem {
   static constexpr int kPanels = D / 64;
   static constexpr uint32_t kQ = 0;
   static constexpr uint32_t kP = kQ + kPanels * kRowPanel;
-  static constexpr uint32_t kK = kP + kRowPanel;              // two stages
-  static constexpr uint32_t kV = kK + 2 * kPanels * kKvPanel;  // two stages
-  static constexpr uint32_t kMisc = kV + 2 * kPanels * kKvPanel;
-  static constexpr uint32_t kBytes = kMisc + 256;
+  static constexpr uint32_t kK = kP + kRowPanel;                     // kStages
+  static constexpr uint32_t kV = kK + kStages * kPanels * kKvPanel;  // kStages
+  static constexpr uint32_t kMisc = kV + kStages * kPanels * kKvPanel;
+  static constexpr uint32_t kMax = kMisc + 256;  // [2 blocks][2 halves][128] row maxima, and at last sums
+  static constexpr uint32_t kFac = kMax + 4 * kRows * 4;  // [128] factors of the rows' scores
+  static constexpr uint32_t kBytes = kFac + kRows * 4;
 };
 
 __device__ __forceinline__ void sts16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Two floats in a register pair, and their sums and products.
+__device__ __forceinline__ uint64_t pack_f2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_f2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 // A page's scale word: K's byte, V's byte, and whether its tokens exist.
@@ -75,21 +111,21 @@ __device__ __forceinline__ int block_parts(const int (&sc)[kPages]) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_kernel(const AttendArgs a) {
   using M = TileMem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + M::kMisc);
-  uint64_t* kv_full = bars;        // [2] K and V of a block written (4 page warps)
-  uint64_t* kv_empty = bars + 2;   // [2] its products are complete (commit)
-  uint64_t* s_full = bars + 4;     // [2] S of a block complete (commit)
-  uint64_t* s_empty = bars + 6;    // [2] S read (4 row warps)
-  uint64_t* q_full = bars + 8;     // Q written (4 row warps)
-  uint64_t* p_full = bars + 9;     // P written (4 row warps)
-  uint64_t* pv_done = bars + 10;   // P V complete (commit)
-  uint64_t* drain = bars + 11;
-  volatile int* scales = reinterpret_cast<int*>(bars + 12);  // [2][kPages]
-  int* misc = reinterpret_cast<int*>(bars + 12) + 2 * kPages;  // [0] abort, [1] TMEM, [2] last of a split tile
+  uint64_t* kv_full = bars;        // [kStages] K and V of a block written (4 page warps)
+  uint64_t* kv_empty = bars + 3;   // [kStages] its products are complete (commit)
+  uint64_t* s_full = bars + 6;     // [2] S of a block complete (commit)
+  uint64_t* s_empty = bars + 8;    // [2] S read (8 row warps)
+  uint64_t* q_full = bars + 10;    // Q written (8 row warps)
+  uint64_t* p_full = bars + 11;    // P written (8 row warps)
+  uint64_t* pv_done = bars + 12;   // P V complete (commit)
+  uint64_t* drain = bars + 13;
+  volatile int* scales = reinterpret_cast<int*>(bars + 14);          // [kStages][kPages]
+  int* misc = reinterpret_cast<int*>(bars + 14) + kStages * kPages;  // [0] abort, [1] TMEM, [2] last of a split tile
   volatile int* abort_flag = misc;
   pdl_wait();
   pdl_trigger();
@@ -102,14 +138,16 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
   const int blocks = (it.pages + kPages - 1) / kPages;
 
   if (tid == 0) {
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       tc::mbar_init(&kv_full[s], 4);
       tc::mbar_init(&kv_empty[s], 1);
-      tc::mbar_init(&s_full[s], 1);
-      tc::mbar_init(&s_empty[s], 4);
     }
-    tc::mbar_init(q_full, 4);
-    tc::mbar_init(p_full, 4);
+    for (int s = 0; s < 2; ++s) {
+      tc::mbar_init(&s_full[s], 1);
+      tc::mbar_init(&s_empty[s], kRowWarps);
+    }
+    tc::mbar_init(q_full, kRowWarps);
+    tc::mbar_init(p_full, kRowWarps);
     tc::mbar_init(pv_done, 1);
     tc::mbar_init(drain, 1);
     misc[0] = 0;
@@ -123,14 +161,15 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = static_cast<uint32_t>(misc[1]);
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return tc::mbar_wait_park_or_abort(bar, parity, a.rows.status, abort_flag);
+  auto wait_ns = [&](uint64_t* bar, uint32_t parity, uint32_t ns) {
+    return tc::mbar_wait_sleep_or_abort(bar, parity, a.rows.status, abort_flag, ns);
   };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_ns(bar, parity, 32); };
 
-  if (warp >= 4) {
+  if (warp >= kRowWarps) {
     // ---------------- pages: codes to f16 tiles; products ----------------
     // Warp w takes page w of every block; ids and scales 32 blocks at a time.
-    const int w = warp - 4;
+    const int w = warp - kRowWarps;
     const uint8_t* head_k = a.cache.data + (int64_t)head * IMBA_PAGE_TOKENS * D;
     const uint8_t* head_v = a.cache.data + a.cache.v_offset + (int64_t)head * IMBA_PAGE_TOKENS * D;
     constexpr int kLoads = D / 32;  // 16-byte loads of a lane, for K and for V
@@ -166,19 +205,19 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
         vr[j] = __ldcg(reinterpret_cast<const uint4*>(head_v + off) + j * 32 + lane);
       }
     };
-    // The products (warp 7, lane 0).
+    // The products (warp 11, lane 0).
     constexpr uint32_t idS = idesc_f16(kRows, kKeys);
     constexpr uint32_t idPV = idesc_f16(kRows, 64) | tc::kIdescBMajorMN;
     uint32_t pv = 0;  // P V issued
     auto issue_s = [&](int b) {
-      const int s = b & 1;
+      const int s = b & 1, kv = b % kStages;
       if (b == 0 && !wait(q_full, 0)) return false;
-      if (!wait(&kv_full[s], (b / 2) & 1) || (b >= 2 && !wait(&s_empty[s], (b / 2 - 1) & 1))) return false;
+      if (!wait(&kv_full[kv], (b / kStages) & 1) || (b >= 2 && !wait(&s_empty[s], (b / 2 - 1) & 1))) return false;
       tc::fence_after_sync();
 #pragma unroll
       for (int n = 0; n < M::kPanels; ++n) {
         const uint64_t dQ = tc::smem_desc_k128(sm + M::kQ + n * kRowPanel);
-        const uint64_t dK = tc::smem_desc_k128(sm + M::kK + (s * M::kPanels + n) * kKvPanel);
+        const uint64_t dK = tc::smem_desc_k128(sm + M::kK + (kv * M::kPanels + n) * kKvPanel);
 #pragma unroll
         for (int k = 0; k < 4; ++k) tc::umma_f16(tmem + 64 * s, dQ + 2 * k, dK + 2 * k, idS, (n | k) != 0);
       }
@@ -186,9 +225,10 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
       return true;
     };
     auto issue_pv = [&](int b) {
+      const int kv = b % kStages;
       int sc4[kPages];
 #pragma unroll
-      for (int p = 0; p < kPages; ++p) sc4[p] = scales[(b & 1) * kPages + p];
+      for (int p = 0; p < kPages; ++p) sc4[p] = scales[kv * kPages + p];
       const int parts = block_parts(sc4);
       const uint64_t dP = tc::smem_desc_k128(sm + M::kP);
       for (int i = 0; i < parts; ++i, ++pv) {
@@ -196,12 +236,12 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
         tc::fence_after_sync();
 #pragma unroll
         for (int n = 0; n < M::kPanels; ++n) {
-          const uint64_t dV = tc::smem_desc_k128(sm + M::kV + ((b & 1) * M::kPanels + n) * kKvPanel);
+          const uint64_t dV = tc::smem_desc_k128(sm + M::kV + (kv * M::kPanels + n) * kKvPanel);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             tc::umma_f16(tmem + 128 + 64 * n, dP + 2 * k, dV + 128 * k, idPV, (pv | k) != 0);
         }
-        if (i + 1 == parts) tc::umma_commit(&kv_empty[b & 1]);
+        if (i + 1 == parts) tc::umma_commit(&kv_empty[kv]);
         tc::umma_commit(pv_done);
       }
       return true;
@@ -209,8 +249,16 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
     if (blocks > 0) load(0);
     bool ok = true;
     for (int b = 0; b < blocks; ++b) {
-      const int s = b & 1;
-      if (b >= 2 && !__all_sync(0xffffffffu, wait(&kv_empty[s], (b / 2 - 1) & 1))) break;
+      const int s = b % kStages;
+      // Block b's stage is free when P V of block b - 3 is complete; the warp of
+      // the products issues those, and S of the block before this, first.
+      if (w == 3 && b >= kStages) {
+        if (lane == 0) ok = issue_pv(b - kStages) && issue_s(b - 1);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+      }
+      if (b >= kStages && !__all_sync(0xffffffffu, wait_ns(&kv_empty[s], (b / kStages - 1) & 1, w == 3 ? 32 : 200)))
+        break;
       const uint32_t kt = tc::smem_u32(sm + M::kK + s * M::kPanels * kKvPanel);
       const uint32_t vt = tc::smem_u32(sm + M::kV + s * M::kPanels * kKvPanel);
 #pragma unroll
@@ -241,86 +289,113 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
         }
       }
       if (lane == 0) scales[s * kPages + w] = sc;
-      if (b + 1 < blocks) load(b + 1);  // behind the stores, ahead of the next wait
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&kv_full[s]);
-      if (w == 3) {
-        if (lane == 0) ok = issue_s(b) && (b == 0 || issue_pv(b - 1));
+      if (b + 1 < blocks) load(b + 1);  // (not before the fence, which would wait for it)
+      if (w == 3 && b < kStages - 1) {  // the first two S
+        if (lane == 0) ok = issue_s(b);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
       }
     }
     if (w == 3 && lane == 0) {
-      if (ok && blocks > 0) issue_pv(blocks - 1);
+      // What the loop has left: P V of the last three blocks, S of the last.
+      for (int b = max(blocks - kStages, 0); ok && b < blocks; ++b)
+        ok = issue_pv(b) && (b + 2 >= blocks || b + 2 < kStages - 1 || issue_s(b + 2));
       // Every product issued here completes before TMEM is freed.
       tc::umma_commit(drain);
       tc::mbar_wait_for(drain, 0, a.rows.status, tc::kWaitNs);
     }
     __syncwarp();
   } else {
-    // ---------------- rows: thread = row of the tile ----------------
-    const int4 row = __ldg(reinterpret_cast<const int4*>(a.plan.rows + (size_t)it.tile * kRows) + tid);
-    const uint32_t tl = tmem + ((uint32_t)(32 * warp) << 16);  // this warp's TMEM lanes
-    const uint32_t sw = (uint32_t)(tid & 7);
+    // ---------------- rows ----------------
+    // Warps w and w + 4 share the rows of TMEM lanes 32 w: thread (row, half).
+    const int half = warp / 4, trow = tid % kRows;
+    const int4 row = __ldg(reinterpret_cast<const int4*>(a.plan.rows + (size_t)it.tile * kRows) + trow);
+    const uint32_t tl = tmem + ((uint32_t)(32 * (warp % 4)) << 16);  // this warp's TMEM lanes
+    const uint32_t sw = (uint32_t)(trow & 7);
     const bool biased = a.call.bias != nullptr;
     const float lg = biased ? kLog2e : 1.f, slack = biased ? kSlack / kLog2e : kSlack;
-    const int vis = row.y - it.key0;  // of the item's keys
+    const int vis = row.y - it.key0 - half * kHalf;  // of the item's keys, from this thread's first
     const float* bias = a.call.bias + (int64_t)(head * a.shape.share + row.w) * (2 * a.call.max_pos - 1);
-    const int col0 = it.key0 - row.z + a.call.max_pos - 1, last = 2 * a.call.max_pos - 2;
-    // The query over its power of two, as f16.
-    float fac;
+    const int col0 = it.key0 + half * kHalf - row.z + a.call.max_pos - 1, last = 2 * a.call.max_pos - 2;
+    volatile float* maxima = reinterpret_cast<float*>(sm + M::kMax);
+    auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + warp % 4) : "memory"); };
+    // The queries over their powers of two, as f16: a warp takes sixteen rows,
+    // lanes are (row, eight elements).
     {
-      const bf16* q = static_cast<const bf16*>(a.call.q) + row.x * a.call.q_stride[0] +
-                      (int64_t)(head * a.shape.share + row.w) * a.call.q_stride[1];
-      const bool vec = a.call.q_stride[0] % 4 == 0 && a.call.q_stride[1] % 4 == 0 &&
-                       (reinterpret_cast<uintptr_t>(a.call.q) & 7) == 0;
-      float amax = 0.f;
-#pragma unroll 4
-      for (int e = 0; e < D; e += 4) {
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        if (row.x >= 0) q_load4(q + e, vec, x);
+      constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kPasses = kRows / kRowWarps / kAtOnce;
+      const int e = lane % kLanes * 8;
+      const bool vec = a.call.q_stride[0] % 8 == 0 && a.call.q_stride[1] % 8 == 0 &&
+                       (reinterpret_cast<uintptr_t>(a.call.q) & 15) == 0;
+      uint4 raw[kPasses];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fabsf(x[j]));
-      }
-      const int ex = (int)(__float_as_uint(amax) >> 23);
-      const int e2 = ex == 0 || ex == 255 ? 0 : min(ex - 127, 126);
-      // a negative scale turns the query, so that the factor is not negative
-      const float down = copysignf(__uint_as_float((uint32_t)(127 - e2) << 23), a.call.scale);
-      fac = __uint_as_float((uint32_t)(127 + e2) << 23) * fabsf(a.call.scale) * (biased ? 1.f : kLog2e);
-      const uint32_t qt = tc::smem_u32(sm + M::kQ) + tid * kPanel;
-#pragma unroll 4
-      for (int e = 0; e < D; e += 8) {
-        float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-        if (row.x >= 0) {
-          q_load4(q + e, vec, x);
-          q_load4(q + e + 4, vec, y);
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = warp * (kRows / kRowWarps) + i * kAtOnce + lane / kLanes;
+        const int4 to = __ldg(reinterpret_cast<const int4*>(a.plan.rows + (size_t)it.tile * kRows) + r);
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (to.x < 0) continue;
+        const bf16* q = static_cast<const bf16*>(a.call.q) + to.x * a.call.q_stride[0] +
+                        (int64_t)(head * a.shape.share + to.w) * a.call.q_stride[1] + e;
+        if (vec) {
+          raw[i] = *reinterpret_cast<const uint4*>(q);
+        } else {
+          uint32_t u[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            u[j] = (uint32_t)__bfloat16_as_ushort(q[2 * j]) | (uint32_t)__bfloat16_as_ushort(q[2 * j + 1]) << 16;
+          raw[i] = make_uint4(u[0], u[1], u[2], u[3]);
         }
-        sts16(qt + e / 64 * kRowPanel + (((uint32_t)(e % 64 / 8) ^ sw) << 4), pack_h2(x[0] * down, x[1] * down),
-              pack_h2(x[2] * down, x[3] * down), pack_h2(y[0] * down, y[1] * down), pack_h2(y[2] * down, y[3] * down));
+      }
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = warp * (kRows / kRowWarps) + i * kAtOnce + lane / kLanes;
+        const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        float x[8], amax = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[2 * j] = __uint_as_float(u[j] << 16);
+          x[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+          amax = fmaxf(amax, fmaxf(fabsf(x[2 * j]), fabsf(x[2 * j + 1])));
+        }
+#pragma unroll
+        for (int o = 1; o < kLanes; o *= 2) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const int ex = (int)(__float_as_uint(amax) >> 23);
+        const int e2 = ex == 0 || ex == 255 ? 0 : min(ex - 127, 126);
+        // a negative scale turns the query, so that the factor is not negative
+        const float down = copysignf(__uint_as_float((uint32_t)(127 - e2) << 23), a.call.scale);
+        if (lane % kLanes == 0)
+          reinterpret_cast<float*>(sm + M::kFac)[r] =
+              __uint_as_float((uint32_t)(127 + e2) << 23) * fabsf(a.call.scale) * (biased ? 1.f : kLog2e);
+        sts16(tc::smem_u32(sm + M::kQ) + e / 64 * kRowPanel + r * kPanel + (((uint32_t)(e % 64 / 8) ^ (uint32_t)(r & 7)) << 4),
+              pack_h2(x[0] * down, x[1] * down), pack_h2(x[2] * down, x[3] * down), pack_h2(x[4] * down, x[5] * down),
+              pack_h2(x[6] * down, x[7] * down));
       }
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(q_full);
+      asm volatile("bar.sync 5, 256;" ::: "memory");
     }
+    const float fac = reinterpret_cast<const float*>(sm + M::kFac)[trow];
 
-    const uint32_t pt = tc::smem_u32(sm + M::kP) + tid * kPanel;
+    const uint32_t pt = tc::smem_u32(sm + M::kP) + trow * kPanel;
     float m = -INFINITY, l = 0.f, ref = 0.f;
     int vref = 0, vmost = 0;
     uint32_t pv = 0;  // P written
     bool ok = true;
-    // O times f, once the last P V is complete.
+    // O (this thread's half of its columns) times f, once the last P V is complete.
     auto rescale = [&](float f) {
       if (pv == 0) return true;
       if (!__all_sync(0xffffffffu, wait(pv_done, (pv - 1) & 1))) return false;
       tc::fence_after_sync();
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
+      for (int c = 0; c < D / 2; c += 32) {
         float o[32];
-        tc::tmem_ld32(tl + 128 + c, o);
+        tc::tmem_ld32(tl + 128 + half * (D / 2) + c, o);
 #pragma unroll
         for (int j = 0; j < 32; ++j) o[j] *= f;
-        tc::tmem_st32(tl + 128 + c, o);
+        tc::tmem_st32(tl + 128 + half * (D / 2) + c, o);
       }
       tc::fence_before_sync();
       return true;
@@ -335,30 +410,32 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
     };
     for (int b = 0; b < blocks; ++b) {
       const int s = b & 1;
-      if (!__all_sync(0xffffffffu, wait(&s_full[s], (b / 2) & 1))) {
-        ok = false;
-        break;
+      // After a wait that ran out a warp only meets its partner, block by block.
+      ok = ok && __all_sync(0xffffffffu, wait(&s_full[s], (b / 2) & 1));
+      if (!ok) {
+        pair_sync();
+        continue;
       }
       tc::fence_after_sync();
-      float x[kKeys];
+      float x[kHalf];
       {
-        uint32_t r[4][16];
-#pragma unroll
-        for (int p = 0; p < kPages; ++p) tc::tmem_ld16_async(tl + 64 * s + 16 * p, r[p]);
+        uint32_t r[2][16];
+        tc::tmem_ld16_async(tl + 64 * s + kHalf * half, r[0]);
+        tc::tmem_ld16_async(tl + 64 * s + kHalf * half + 16, r[1]);
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int p = 0; p < kPages; ++p)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) x[16 * p + j] = __uint_as_float(r[p][j]);
+        for (int j = 0; j < kHalf; ++j) x[j] = __uint_as_float(r[j / 16][j % 16]);
       }
       int sc[kPages];
       bool here = true;
-      int top = 0;
+      int top = 0, low = 255;  // of the block's V scales
 #pragma unroll
       for (int p = 0; p < kPages; ++p) {
-        sc[p] = scales[s * kPages + p];
+        sc[p] = scales[b % kStages * kPages + p];
         here &= (sc[p] & kPageHere) != 0;
-        top = max(top, sc[p] >> 8 & 255);
+        const int vb = sc[p] >> 8 & 255;
+        top = max(top, vb);
+        low = min(low, vb ? vb : 255);
       }
       const int parts = block_parts(sc);
       tc::fence_before_sync();
@@ -366,34 +443,37 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
       if (lane == 0) tc::mbar_arrive(&s_empty[s]);
 
       // Scores: x stays raw, with a factor a page, where nothing is added or hidden.
-      float f[kPages], mx = -INFINITY;
+      const int mine[2] = {half ? sc[2] : sc[0], half ? sc[3] : sc[1]};  // this thread's pages
+      float f[2] = {scale_of(mine[0] & 255) * fac, scale_of(mine[1] & 255) * fac};
+      float mx = -INFINITY;
+      if (here && !biased && it.key0 + (b + 1) * kKeys <= it.minvis) {
 #pragma unroll
-      for (int p = 0; p < kPages; ++p) f[p] = scale_of(sc[p] & 255) * fac;
-      const bool plain = here && !biased && it.key0 + (b + 1) * kKeys <= it.minvis;
-      if (plain) {
+        for (int p = 0; p < 2; ++p) {
+          float t = fmaxf(x[16 * p], x[16 * p + 1]);
 #pragma unroll
-        for (int p = 0; p < kPages; ++p) {
-          float t = x[16 * p];
-#pragma unroll
-          for (int j = 1; j < 16; ++j) t = fmaxf(t, x[16 * p + j]);
+          for (int j = 2; j < 16; j += 2) t = max3(t, x[16 * p + j], x[16 * p + j + 1]);
           mx = fmaxf(mx, t * f[p]);
         }
       } else {
         const int nv = vis - b * kKeys;
 #pragma unroll
-        for (int p = 0; p < kPages; ++p) {
-          const bool on = (sc[p] & kPageHere) != 0;
+        for (int p = 0; p < 2; ++p) {
+          const int n = mine[p] & kPageHere ? nv : 0;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             float y = x[16 * p + j] * f[p];
             if (biased) y += take_bias(__ldg(bias + min(max(col0 + b * kKeys + 16 * p + j, 0), last)));
-            y = on && 16 * p + j < nv ? y : -INFINITY;
+            y = 16 * p + j < n ? y : -INFINITY;
             x[16 * p + j] = y;
             mx = fmaxf(mx, y);
           }
           f[p] = 1.f;
         }
       }
+      // The row's maximum over both halves.
+      maxima[(s * 2 + half) * kRows + trow] = mx;
+      pair_sync();
+      mx = fmaxf(mx, maxima[(s * 2 + 1 - half) * kRows + trow]);
       float grow = 1.f;
       if (__any_sync(0xffffffffu, mx > m + slack)) {
         const float now = fmaxf(m, mx);
@@ -402,36 +482,34 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
         ref = now == -INFINITY ? 0.f : fmaf(-now, lg, kShift);
         l *= grow;
       }
-      if (parts == 1 && top) {
-        int low = 255;
-#pragma unroll
-        for (int p = 0; p < kPages; ++p) low = min(low, sc[p] >> 8 & 255 ? sc[p] >> 8 & 255 : 255);
-        // the middle of the block's scales: both ends stay inside the window
-        if (vref == 0 || top - vref > kVWindow || vref - low > kVWindow) grow *= set_units((top + low) / 2);
-      }
+      // the middle of the block's scales: both ends stay inside the window
+      if (parts == 1 && top && (vref == 0 || top - vref > kVWindow || vref - low > kVWindow))
+        grow *= set_units((top + low) / 2);
       if (__any_sync(0xffffffffu, grow != 1.f) && !rescale(grow)) {
         ok = false;
-        break;
+        continue;
       }
-      // Weights, four pages of sixteen, as f16 pairs.
-      uint32_t w[kKeys / 2];
+      // Weights, two pages of sixteen, as f16 pairs.
+      uint32_t w[kHalf / 2];
 #pragma unroll
-      for (int p = 0; p < kPages; ++p) {
-        const int vb = sc[p] >> 8 & 255;
+      for (int p = 0; p < 2; ++p) {
+        const int vb = mine[p] >> 8 & 255;
         const int up = parts == 1 && vb ? min(max(vb - vref, -126), kVWindow) : 0;
         const float from = ref + (float)up, by = f[p] * lg;
-        float sum = 0.f;
+        const uint64_t from2 = pack_f2(from, from), by2 = pack_f2(by, by);
+        uint64_t sum = 0;
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-          const float e0 = exp2_approx(fmaf(x[16 * p + j], by, from));
-          const float e1 = exp2_approx(fmaf(x[16 * p + j + 1], by, from));
-          sum += e0 + e1;
+          const float2 z = unpack_f2(fma_f2(pack_f2(x[16 * p + j], x[16 * p + j + 1]), by2, from2));
+          const float e0 = exp2_approx(z.x), e1 = exp2_approx(z.y);
+          sum = add_f2(sum, pack_f2(e0, e1));
           w[8 * p + j / 2] = pack_h2(e0, e1);
         }
-        l = fmaf(sum, __uint_as_float((uint32_t)(127 - up) << 23), l);
+        const float2 both = unpack_f2(sum);
+        l = fmaf(both.x + both.y, __uint_as_float((uint32_t)(127 - up) << 23), l);
       }
-      for (int i = 0; i < parts && ok; ++i) {
-        bool mine = true;
+      for (int i = 0; i < parts; ++i) {
+        bool on = true;
         if (parts > 1) {  // page i alone, in units of its own scale
           int vb = 0;
 #pragma unroll
@@ -443,30 +521,31 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
               break;
             }
           }
-          mine = vb == vref;  // (else far below the largest scale, or zeros)
+          on = vb == vref;  // (else far below the largest scale, or zeros)
         }
         if (pv > 0 && !__all_sync(0xffffffffu, wait(pv_done, (pv - 1) & 1))) {  // P is free
           ok = false;
           break;
         }
 #pragma unroll
-        for (int c = 0; c < kKeys / 8; ++c) {
-          const bool on = parts == 1 || (mine && c / 2 == i);
-          uint32_t u[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) u[j] = on ? w[4 * c + j] : 0u;
-          sts16(pt + (((uint32_t)c ^ sw) << 4), u[0], u[1], u[2], u[3]);
+        for (int c = 0; c < 4; ++c) {
+          uint32_t u[4] = {w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]};
+          if (parts > 1 && !(on && 2 * half + c / 2 == i)) u[0] = u[1] = u[2] = u[3] = 0;
+          sts16(pt + (((uint32_t)(4 * half + c) ^ sw) << 4), u[0], u[1], u[2], u[3]);
         }
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(p_full);
         ++pv;
       }
-      if (!ok) break;
     }
     if (ok && pv > 0) ok = __all_sync(0xffffffffu, wait(pv_done, (pv - 1) & 1));
     tc::fence_after_sync();
-    const size_t part = ((size_t)max(it.part, 0) * H + head) * kRows + tid;
+    asm volatile("bar.sync 5, 256;" ::: "memory");  // all rows' maxima have been read
+    maxima[half * kRows + trow] = l;
+    asm volatile("bar.sync 5, 256;" ::: "memory");
+    l += maxima[(1 - half) * kRows + trow];
+    const size_t part = ((size_t)max(it.part, 0) * H + head) * kRows + trow;
     const float unit_v = vref ? scale_of(vref) : 1.f;
     const float f = it.part >= 0 ? unit_v : l == 0.f ? 0.f : unit_v / l;
     const bool ovec = a.call.out_stride[0] % 4 == 0 && a.call.out_stride[1] % 4 == 0 &&
@@ -474,9 +553,9 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
     bf16* out = static_cast<bf16*>(a.call.out) + row.x * a.call.out_stride[0] +
                 (int64_t)(head * a.shape.share + row.w) * a.call.out_stride[1];
     if (ok) {
-      if (it.part >= 0 && row.x >= 0) a.plan.ml[part] = make_float2(m, l);
+      if (it.part >= 0 && row.x >= 0 && half == 0) a.plan.ml[part] = make_float2(m, l);
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
+      for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
         float o[32];
         if (pv > 0) {
           tc::tmem_ld32(tl + 128 + c, o);
@@ -498,14 +577,14 @@ __global__ void __launch_bounds__(kTileThreads, 2) attend8_tile_kernel(const Att
     }
     if (it.part >= 0) {  // (after a wait that ran out too: the counter is left as it was found)
       __threadfence();
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      int* done = a.plan.done + (size_t)it.tile * H + head;
+      asm volatile("bar.sync 5, 256;" ::: "memory");
+      int* done = a.plan.done + ((size_t)it.tile * H + head) * 8;
       if (tid == 0) misc[2] = atomicAdd(done, 1) == it.splits - 1;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      asm volatile("bar.sync 5, 256;" ::: "memory");
       if (misc[2]) {
         __threadfence();
         if (tid == 0) *done = 0;
-        join_items<bf16, D>(a, it, head, lg, 0, kRows, tid, kRows);
+        join_items<bf16, D>(a, it, head, lg, 0, kRows, tid, 2 * kRows);
       }
     }
     tc::fence_before_sync();

@@ -116,6 +116,28 @@ __device__ __forceinline__ bool mbar_wait_park_or_abort(uint64_t* bar, uint32_t 
   }
 }
 
+// mbar_wait_or_abort with a sleep of `ns` between polls and the clock read at
+// every 64th of them only: a poll with the clock costs some twenty issue
+// slots, which a kernel with many waiting warps takes from those that work.
+__device__ __forceinline__ bool mbar_wait_sleep_or_abort(uint64_t* bar, uint32_t parity, int32_t* status,
+                                                         volatile int* abort, uint32_t ns) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_ns();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i) {
+      __nanosleep(ns);
+      if (mbar_try_wait(bar, parity)) return true;
+    }
+    if (*abort) return false;
+    if (global_ns() - t0 > kWaitNs) {
+      report(status, IMBA_ERR_TIMEOUT);
+      *abort = 1;
+      return false;
+    }
+  }
+}
+
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
