@@ -58,10 +58,12 @@ struct TileMem {
   static constexpr uint32_t kK = kP + kRowPanel;                     // kStages
   static constexpr uint32_t kV = kK + kStages * kPanels * kKvPanel;  // kStages
   static constexpr uint32_t kMisc = kV + kStages * kPanels * kKvPanel;
-  static constexpr uint32_t kMax = kMisc + 256;  // [2 blocks][2 halves][128] row maxima, and at last sums
+  static constexpr uint32_t kInfo = kMisc + 256;
+  static constexpr uint32_t kMax = kInfo + 512;  // [2 blocks][2 halves][128] row maxima, and at last sums
   static constexpr uint32_t kFac = kMax + 4 * kRows * 4;  // [128] factors of the rows' scores
   static constexpr uint32_t kBytes = kFac + kRows * 4;
 };
+
 
 __device__ __forceinline__ void sts16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -95,20 +97,74 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// A page's scale word: K's byte, V's byte, and whether its tokens exist.
-constexpr int kPageHere = 1 << 16;
+// What the rows have to know of a block, written by a page warp beside its
+// tiles.  V's units (the scale byte that O is held in units of) follow the
+// blocks' scales and are the same for every row, so they are kept there.
+struct BlockInfo {
+  float ks[kPages];    // K's scales
+  float up[kPages];    // log2 of V's scales in units of O
+  float down[kPages];  // 2^-up
+  float turn[kPages];  // with parts: what O is multiplied by before each page's P V
+  float grow;          // without: what O is multiplied by
+  int here;            // every page exists
+  int parts;           // P V of the block: 1, or one a page
+  int on;              // with parts: the pages that are not far below the largest scale (bits)
+  float unit;          // O's units after the block
+  int pages;           // the pages that exist (bits)
+};
 
-// How many P V a block takes: one, or one a page.
-__device__ __forceinline__ int block_parts(const int (&sc)[kPages]) {
-  int top = 0, low = 255;
-#pragma unroll
-  for (int p = 0; p < kPages; ++p) {
-    const int vb = sc[p] >> 8 & 255;
-    top = max(top, vb);
-    low = min(low, vb ? vb : 255);
+static_assert(kStages * sizeof(BlockInfo) <= 512, "BlockInfo's place in shared memory");
+
+// The scale byte that O is held in units of.
+struct Units {
+  int vref = 0, vmost = 0;
+  // To byte vb, as near as 2^80 of the largest so far lets it be (no sum then
+  // overflows); what O is multiplied by.
+  __device__ __forceinline__ float set(int vb) {
+    vmost = max(vmost, vb);
+    const int now = max(vb, vmost - 80), by = vref ? vref - now : 0;
+    vref = now;
+    return by < -126 ? 0.f : __uint_as_float((uint32_t)(127 + by) << 23);
   }
-  return top - low > kSpread && low < 255 ? kPages : 1;
-}
+  // The next block, its pages' scale bytes K | V << 8 (-1: no page).
+  __device__ __forceinline__ void next(const int (&sc)[kPages], BlockInfo& o) {
+    int top = 0, low = 255;
+    o.pages = 0;
+#pragma unroll
+    for (int p = 0; p < kPages; ++p) {
+      const int vb = sc[p] < 0 ? 0 : sc[p] >> 8;
+      o.ks[p] = sc[p] < 0 ? 0.f : scale_of(sc[p] & 255);
+      o.pages |= (sc[p] >= 0) << p;
+      top = max(top, vb);
+      low = min(low, vb ? vb : 255);
+      o.up[p] = 0.f;
+      o.down[p] = o.turn[p] = 1.f;
+    }
+    o.here = o.pages == (1 << kPages) - 1;
+    o.parts = top - low > kSpread ? kPages : 1;  // (top 0: low is 255)
+    o.on = 0;
+    o.grow = 1.f;
+    if (o.parts == 1) {
+      // the middle of the block's scales: both ends stay inside the window
+      if (top && (vref == 0 || top - vref > kVWindow || vref - low > kVWindow)) o.grow = set((top + low) / 2);
+#pragma unroll
+      for (int p = 0; p < kPages; ++p) {
+        const int vb = sc[p] < 0 ? 0 : sc[p] >> 8;
+        const int up = vb ? min(max(vb - vref, -126), kVWindow) : 0;
+        o.up[p] = (float)up;
+        o.down[p] = __uint_as_float((uint32_t)(127 - up) << 23);
+      }
+    } else {
+#pragma unroll
+      for (int p = 0; p < kPages; ++p) {
+        const int vb = sc[p] < 0 ? 0 : sc[p] >> 8;
+        if (vb) o.turn[p] = set(vb);
+        o.on |= (vb != 0 && vb == vref) << p;
+      }
+    }
+    o.unit = vref ? scale_of(vref) : 1.f;
+  }
+};
 
 template <int D>
 __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_kernel(const AttendArgs a) {
@@ -124,8 +180,8 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
   uint64_t* p_full = bars + 11;    // P written (8 row warps)
   uint64_t* pv_done = bars + 12;   // P V complete (commit)
   uint64_t* drain = bars + 13;
-  volatile int* scales = reinterpret_cast<int*>(bars + 14);          // [kStages][kPages]
-  int* misc = reinterpret_cast<int*>(bars + 14) + kStages * kPages;  // [0] abort, [1] TMEM, [2] last of a split tile
+  int* misc = reinterpret_cast<int*>(bars + 14);  // [0] abort, [1] TMEM, [2] last of a split tile
+  BlockInfo* infos = reinterpret_cast<BlockInfo*>(sm + M::kInfo);  // [kStages]
   volatile int* abort_flag = misc;
   pdl_wait();
   pdl_trigger();
@@ -173,28 +229,35 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
     const uint8_t* head_k = a.cache.data + (int64_t)head * IMBA_PAGE_TOKENS * D;
     const uint8_t* head_v = a.cache.data + a.cache.v_offset + (int64_t)head * IMBA_PAGE_TOKENS * D;
     constexpr int kLoads = D / 32;  // 16-byte loads of a lane, for K and for V
-    int id32 = -1, sc32 = 0;
-    auto fetch_ids = [&](int b0) {  // lane: page of block b0 + lane
-      const int p = (b0 + lane) * kPages + w;
-      id32 = -1;
-      sc32 = 0;
-      if (p < it.pages) {
-        const int id = a.rows.group_pages[it.list + p];
-        if (id >= 0 && id < a.cache.num_pages) {
-          id32 = id;
-          const uint8_t* s = a.cache.scales + id * a.cache.scale_stride + head;
-          sc32 = s[0] | s[H] << 8 | kPageHere;
-        } else {
-          report(a.rows.status, IMBA_ERR_RANGE);
+    int id32 = -1;
+    int sc32[kPages];  // the first page warp: scale bytes of the block's pages, -1 for none
+    Units units;
+    auto page_at = [&](int p) {
+      const int id = p < it.pages ? a.rows.group_pages[it.list + p] : -1;
+      if (p < it.pages && (id < 0 || id >= a.cache.num_pages)) {
+        report(a.rows.status, IMBA_ERR_RANGE);
+        return -1;
+      }
+      return id;
+    };
+    auto fetch_ids = [&](int b0) {  // lane: block b0 + lane
+      if (w == 0) {
+        int id[kPages];
+#pragma unroll
+        for (int p = 0; p < kPages; ++p) id[p] = page_at((b0 + lane) * kPages + p);
+        id32 = id[0];
+#pragma unroll
+        for (int p = 0; p < kPages; ++p) {
+          const uint8_t* s = a.cache.scales + max(id[p], 0) * a.cache.scale_stride + head;
+          sc32[p] = id[p] < 0 ? -1 : s[0] | s[H] << 8;
         }
+      } else {
+        id32 = page_at((b0 + lane) * kPages + w);
       }
     };
     uint4 kr[kLoads], vr[kLoads];
-    int sc = 0;
     auto load = [&](int b) {
-      if ((b & 31) == 0) fetch_ids(b);
       const int id = __shfl_sync(0xffffffffu, id32, b & 31);
-      sc = __shfl_sync(0xffffffffu, sc32, b & 31);
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) kr[j] = vr[j] = make_uint4(0, 0, 0, 0);
       if (id < 0) return;
@@ -226,10 +289,7 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
     };
     auto issue_pv = [&](int b) {
       const int kv = b % kStages;
-      int sc4[kPages];
-#pragma unroll
-      for (int p = 0; p < kPages; ++p) sc4[p] = scales[kv * kPages + p];
-      const int parts = block_parts(sc4);
+      const int parts = *reinterpret_cast<volatile int*>(&infos[kv].parts);
       const uint64_t dP = tc::smem_desc_k128(sm + M::kP);
       for (int i = 0; i < parts; ++i, ++pv) {
         if (!wait(p_full, pv & 1)) return false;
@@ -246,6 +306,7 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
       }
       return true;
     };
+    fetch_ids(0);
     if (blocks > 0) load(0);
     bool ok = true;
     for (int b = 0; b < blocks; ++b) {
@@ -288,11 +349,21 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
           sts16(dst + kPanel + ((c ^ ((row + 1) & 7)) << 4), h[0], h[1], h[2], h[3]);
         }
       }
-      if (lane == 0) scales[s * kPages + w] = sc;
+      if (w == 0) {
+        int sc[kPages];
+#pragma unroll
+        for (int p = 0; p < kPages; ++p) sc[p] = __shfl_sync(0xffffffffu, sc32[p], b & 31);
+        BlockInfo info;
+        units.next(sc, info);
+        if (lane == 0) infos[s] = info;
+      }
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&kv_full[s]);
-      if (b + 1 < blocks) load(b + 1);  // (not before the fence, which would wait for it)
+      if (b + 1 < blocks) {  // (not before the fence, which would wait for it)
+        if (((b + 1) & 31) == 0) fetch_ids(b + 1);
+        load(b + 1);
+      }
       if (w == 3 && b < kStages - 1) {  // the first two S
         if (lane == 0) ok = issue_s(b);
         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -381,8 +452,8 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
 
     const uint32_t pt = tc::smem_u32(sm + M::kP) + trow * kPanel;
     float m = -INFINITY, l = 0.f, ref = 0.f;
-    int vref = 0, vmost = 0;
-    uint32_t pv = 0;  // P written
+    float unit = 1.f;  // O's
+    uint32_t pv = 0;   // P written
     bool ok = true;
     // O (this thread's half of its columns) times f, once the last P V is complete.
     auto rescale = [&](float f) {
@@ -400,14 +471,9 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
       tc::fence_before_sync();
       return true;
     };
-    // O's units to V scale byte vb, as near as 2^80 of the largest so far lets
-    // them be (the same for all rows); what O is to be multiplied by.
-    auto set_units = [&](int vb) -> float {
-      vmost = max(vmost, vb);
-      const int now = max(vb, vmost - 80), by = vref ? vref - now : 0;
-      vref = now;
-      return by < -126 ? 0.f : __uint_as_float((uint32_t)(127 + by) << 23);
-    };
+    uint32_t at[4];  // this thread's chunks of P
+#pragma unroll
+    for (int c = 0; c < 4; ++c) at[c] = pt + (((uint32_t)(4 * half + c) ^ sw) << 4);
     for (int b = 0; b < blocks; ++b) {
       const int s = b & 1;
       // After a wait that ran out a warp only meets its partner, block by block.
@@ -426,25 +492,19 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
 #pragma unroll
         for (int j = 0; j < kHalf; ++j) x[j] = __uint_as_float(r[j / 16][j % 16]);
       }
-      int sc[kPages];
-      bool here = true;
-      int top = 0, low = 255;  // of the block's V scales
-#pragma unroll
-      for (int p = 0; p < kPages; ++p) {
-        sc[p] = scales[b % kStages * kPages + p];
-        here &= (sc[p] & kPageHere) != 0;
-        const int vb = sc[p] >> 8 & 255;
-        top = max(top, vb);
-        low = min(low, vb ? vb : 255);
-      }
-      const int parts = block_parts(sc);
+      const BlockInfo& info = infos[b % kStages];
+      const float2 ks = *reinterpret_cast<const float2*>(info.ks + 2 * half);
+      const float2 up = *reinterpret_cast<const float2*>(info.up + 2 * half);
+      const float2 down = *reinterpret_cast<const float2*>(info.down + 2 * half);
+      const float turned = info.grow;
+      const int here = info.here, parts = info.parts;
+      unit = info.unit;
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&s_empty[s]);
 
       // Scores: x stays raw, with a factor a page, where nothing is added or hidden.
-      const int mine[2] = {half ? sc[2] : sc[0], half ? sc[3] : sc[1]};  // this thread's pages
-      float f[2] = {scale_of(mine[0] & 255) * fac, scale_of(mine[1] & 255) * fac};
+      float f[2] = {ks.x * fac, ks.y * fac};
       float mx = -INFINITY;
       if (here && !biased && it.key0 + (b + 1) * kKeys <= it.minvis) {
 #pragma unroll
@@ -458,7 +518,7 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
         const int nv = vis - b * kKeys;
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const int n = mine[p] & kPageHere ? nv : 0;
+          const int n = info.pages >> (2 * half + p) & 1 ? nv : 0;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             float y = x[16 * p + j] * f[p];
@@ -474,28 +534,21 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
       maxima[(s * 2 + half) * kRows + trow] = mx;
       pair_sync();
       mx = fmaxf(mx, maxima[(s * 2 + 1 - half) * kRows + trow]);
-      float grow = 1.f;
-      if (__any_sync(0xffffffffu, mx > m + slack)) {
-        const float now = fmaxf(m, mx);
-        grow = weight_of(m, now, lg);
+      if (__any_sync(0xffffffffu, mx > m + slack) || turned != 1.f) {
+        const float now = fmaxf(m, mx), w = weight_of(m, now, lg);
         m = now;
         ref = now == -INFINITY ? 0.f : fmaf(-now, lg, kShift);
-        l *= grow;
-      }
-      // the middle of the block's scales: both ends stay inside the window
-      if (parts == 1 && top && (vref == 0 || top - vref > kVWindow || vref - low > kVWindow))
-        grow *= set_units((top + low) / 2);
-      if (__any_sync(0xffffffffu, grow != 1.f) && !rescale(grow)) {
-        ok = false;
-        continue;
+        l *= w;
+        if (!rescale(w * turned)) {
+          ok = false;
+          continue;
+        }
       }
       // Weights, two pages of sixteen, as f16 pairs.
       uint32_t w[kHalf / 2];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const int vb = mine[p] >> 8 & 255;
-        const int up = parts == 1 && vb ? min(max(vb - vref, -126), kVWindow) : 0;
-        const float from = ref + (float)up, by = f[p] * lg;
+        const float from = ref + (p ? up.y : up.x), by = f[p] * lg;
         const uint64_t from2 = pack_f2(from, from), by2 = pack_f2(by, by);
         uint64_t sum = 0;
 #pragma unroll
@@ -506,32 +559,31 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
           w[8 * p + j / 2] = pack_h2(e0, e1);
         }
         const float2 both = unpack_f2(sum);
-        l = fmaf(both.x + both.y, __uint_as_float((uint32_t)(127 - up) << 23), l);
+        l = fmaf(both.x + both.y, p ? down.y : down.x, l);
       }
       for (int i = 0; i < parts; ++i) {
-        bool on = true;
+        bool all = true;
         if (parts > 1) {  // page i alone, in units of its own scale
-          int vb = 0;
-#pragma unroll
-          for (int p = 0; p < kPages; ++p) vb = p == i ? sc[p] >> 8 & 255 : vb;
-          if (vb) {
-            const float g = set_units(vb);
-            if (g != 1.f && !rescale(g)) {
-              ok = false;
-              break;
-            }
+          const float turn = info.turn[i];
+          if (turn != 1.f && !rescale(turn)) {
+            ok = false;
+            break;
           }
-          on = vb == vref;  // (else far below the largest scale, or zeros)
+          all = false;
         }
         if (pv > 0 && !__all_sync(0xffffffffu, wait(pv_done, (pv - 1) & 1))) {  // P is free
           ok = false;
           break;
         }
+        if (all) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t u[4] = {w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]};
-          if (parts > 1 && !(on && 2 * half + c / 2 == i)) u[0] = u[1] = u[2] = u[3] = 0;
-          sts16(pt + (((uint32_t)(4 * half + c) ^ sw) << 4), u[0], u[1], u[2], u[3]);
+          for (int c = 0; c < 4; ++c) sts16(at[c], w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const bool on = 2 * half + c / 2 == i && (info.on >> i & 1);
+            sts16(at[c], on ? w[4 * c] : 0, on ? w[4 * c + 1] : 0, on ? w[4 * c + 2] : 0, on ? w[4 * c + 3] : 0);
+          }
         }
         tc::fence_proxy_async_smem();
         __syncwarp();
@@ -546,8 +598,7 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
     asm volatile("bar.sync 5, 256;" ::: "memory");
     l += maxima[(1 - half) * kRows + trow];
     const size_t part = ((size_t)max(it.part, 0) * H + head) * kRows + trow;
-    const float unit_v = vref ? scale_of(vref) : 1.f;
-    const float f = it.part >= 0 ? unit_v : l == 0.f ? 0.f : unit_v / l;
+    const float f = it.part >= 0 ? unit : l == 0.f ? 0.f : unit / l;
     const bool ovec = a.call.out_stride[0] % 4 == 0 && a.call.out_stride[1] % 4 == 0 &&
                       (reinterpret_cast<uintptr_t>(a.call.out) & 7) == 0;
     bf16* out = static_cast<bf16*>(a.call.out) + row.x * a.call.out_stride[0] +
