@@ -15,6 +15,12 @@ constexpr int kTileRows = 8;
 constexpr int kUnitWarps = 8;  // warps of a CTA
 constexpr int kTileGroups = 16;  // rt of the tcgen05 kernel's tiles of 128 rows
 
+// CTAs an SM, by what a lane's rows take in registers (tcgen05: by TMEM and
+// the operands in shared memory).
+constexpr int attend8_ctas(int dqk, int rt) {
+  return rt == kTileGroups ? 2 : dqk > 64 ? (rt == 1 ? 2 : 1) : rt == 1 ? 3 : 2;
+}
+
 struct AttendRow {  // one flattened row of a tile
   int row;          // -1: none
   int vis;          // visible tokens of the page list

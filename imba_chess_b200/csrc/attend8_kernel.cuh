@@ -724,9 +724,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
 template <typename T, int DQK, int DV, int RT, int NW>
 cudaError_t launch_one(const AttendArgs& a, cudaStream_t s) {
   using D = Dims<DQK, DV, RT>;
-  constexpr int kStages = 3;
-  // CTAs an SM by what a lane's rows take in registers
-  constexpr int kCtas = DQK > 64 ? (RT == 1 ? 2 : 1) : RT == 1 ? 3 : 2;
+  constexpr int kCtas = attend8_ctas(DQK, RT), kStages = 3;
   constexpr size_t ring = (size_t)kUnitWarps * kStages * D::STAGE;
   constexpr size_t smem = NW > 1 && D::MERGE > ring ? D::MERGE : ring;
   auto fn = attend8_kernel<T, DQK, DV, RT, NW, kStages, kCtas>;

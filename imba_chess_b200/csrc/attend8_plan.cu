@@ -214,7 +214,7 @@ AttendShape shape_of(const imba_cache_desc& c, const imba_attend_desc& r, int rt
   // About four CTAs' worth of units for each that is resident (two of the
   // tcgen05 kernel's, whose parts are large).
   const int waves = rt == kTileGroups ? 2 : 4;
-  sh.target = (int)std::min<int64_t>(most, std::max(1, 148 * 2 * waves * (kUnitWarps / warps) / c.num_heads));
+  sh.target = (int)std::min<int64_t>(most, std::max(1, 148 * std::min(attend8_ctas(c.attention_dim, rt), 2) * waves * (kUnitWarps / warps) / c.num_heads));
   const int64_t by_len = (int64_t)sh.max_tiles * ((r.num_group_pages + sh.min_pages - 1) / sh.min_pages);
   const int64_t cut = std::min<int64_t>(by_len, sh.target);  // full-size items; each tile may add one smaller
   sh.max_items = (int)std::min<int64_t>(sh.max_tiles + cut, INT32_MAX / 4);
