@@ -18,7 +18,7 @@ constexpr int kTileGroups = 16;  // rt of the tcgen05 kernel's tiles of 128 rows
 // CTAs an SM, by what a lane's rows take in registers (tcgen05: by TMEM and
 // the operands in shared memory).
 constexpr int attend8_ctas(int dqk, int rt) {
-  return rt == kTileGroups ? 2 : dqk > 64 ? (rt == 1 ? 2 : 1) : rt == 1 ? 3 : 2;
+  return rt == kTileGroups ? 2 : dqk > 64 ? (rt == 1 ? 2 : 1) : rt == 1 ? 3 : rt == 2 || dqk == 32 ? 2 : 1;
 }
 
 struct AttendRow {  // one flattened row of a tile
@@ -40,7 +40,7 @@ struct AttendItem {
 
 struct AttendShape {
   int share;        // query heads per key / value head
-  int rt;           // 8-row groups of a tile: 1, 2 or kTileGroups
+  int rt;           // 8-row groups of a tile: 1, 2, 3 or kTileGroups
   int warps;        // warps that share a unit: 1 or kUnitWarps
   int tile_rows;    // kTileRows * rt
   int max_tiles;

@@ -216,7 +216,8 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
   const int sub = NW == 1 ? 0 : warp;
   const int H = a.cache.H;
   const uint32_t unit = NW == 1 ? blockIdx.x * kUnitWarps + warp : blockIdx.x;
-  // (a plan with tiles of 128 rows: eight units of sixteen a tile)
+  // (fp32 rows on a plan with tiles of 128 or 24 rows: eight units of 16 a
+  // tile, or three of eight)
   const int subs = a.shape.tile_rows / D::ROWS, sub_tile = subs > 1 ? (int)(unit % (uint32_t)subs) : 0;
   const uint32_t whole = subs > 1 ? unit / (uint32_t)subs : unit;
   const int item_id = (int)(whole / (uint32_t)H), head = (int)(whole % (uint32_t)H);
@@ -650,7 +651,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
       if (__shfl_sync(0xffffffffu, n, 0) == it.splits - 1) {  // the others have finished
         __threadfence();
         if (lane == 0) *done = 0;
-        join_items<T, DV>(a, it, head, st.lg, r0, D::ROWS, lane, 32);
+        join_items<T, DV, 8>(a, it, head, st.lg, r0, D::ROWS, lane, 32);
       }
     }
   } else {
@@ -715,7 +716,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
       if (*flag) {
         __threadfence();
         if (threadIdx.x == 0) *done = 0;
-        join_items<T, DV>(a, it, head, st.lg, r0, D::ROWS, threadIdx.x, kUnitWarps * 32);
+        join_items<T, DV, 8>(a, it, head, st.lg, r0, D::ROWS, threadIdx.x, kUnitWarps * 32);
       }
     }
   }
@@ -743,12 +744,18 @@ cudaError_t launch_rows(const AttendArgs& a, cudaStream_t s) {
 
 }  // namespace
 
+// 24 rows of queries as two f16 parts do not fit the registers: fp32 takes
+// such a tile as three of eight.
+template <typename T>
+constexpr int kThree = sizeof(T) == 2 ? 3 : 1;
+
 template <typename T>
 cudaError_t launch_attend8(const imba_cache_desc& c, const AttendArgs& a, cudaStream_t s) {
   if (a.shape.rt == kTileGroups && sizeof(T) == 2) return launch_attend8_tile(c, a, s);
 #define IMBA_ATTEND8(DQK, DV)                                              \
   if (c.attention_dim == DQK && c.linear_dim == DV) {                      \
     if (a.shape.rt == 1) return launch_rows<T, DQK, DV, 1>(a, s);          \
+    if (a.shape.rt == 3) return launch_rows<T, DQK, DV, kThree<T>>(a, s);  \
     return launch_rows<T, DQK, DV, 2>(a, s);                               \
   }
   IMBA_ATTEND8(32, 32)

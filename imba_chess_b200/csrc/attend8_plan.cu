@@ -212,9 +212,12 @@ AttendShape shape_of(const imba_cache_desc& c, const imba_attend_desc& r, int rt
   sh.warps = warps;
   sh.min_pages = warps == 1 ? 16 : 8;
   // About four CTAs' worth of units for each that is resident (two of the
-  // tcgen05 kernel's, whose parts are large).
-  const int waves = rt == kTileGroups ? 2 : 4;
-  sh.target = (int)std::min<int64_t>(most, std::max(1, 148 * std::min(attend8_ctas(c.attention_dim, rt), 2) * waves * (kUnitWarps / warps) / c.num_heads));
+  // tcgen05 kernel's, whose parts are large), but fewer for a step of few
+  // tiles, so that one is not joined from more than about 32 parts.
+  const int ctas = std::min(attend8_ctas(c.attention_dim, rt), 2);
+  const int64_t few = std::max<int64_t>((flat + sh.tile_rows - 1) / sh.tile_rows, r.num_segs) * c.num_heads * 32;
+  const int waves = (int)std::min<int64_t>(rt == kTileGroups ? 2 : 4, std::max<int64_t>(1, few / (148 * ctas)));
+  sh.target = (int)std::min<int64_t>(most, std::max(1, 148 * ctas * waves * (kUnitWarps / warps) / c.num_heads));
   const int64_t by_len = (int64_t)sh.max_tiles * ((r.num_group_pages + sh.min_pages - 1) / sh.min_pages);
   const int64_t cut = std::min<int64_t>(by_len, sh.target);  // full-size items; each tile may add one smaller
   sh.max_items = (int)std::min<int64_t>(sh.max_tiles + cut, INT32_MAX / 4);
@@ -230,7 +233,11 @@ AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r, in
   const int64_t per_seg = r.num_segs ? (flat + r.num_segs - 1) / r.num_segs : 0;
   if (r.num_extra == 0 && c.attention_dim == c.linear_dim && c.attention_dim % 64 == 0 && per_seg >= kTileFrom)
     return shape_of(c, r, kTileGroups, kUnitWarps, most);
-  const int rt = per_seg <= 8 ? 1 : 2;
+  // Three groups only where they save a tile of two (20 rows a segment, bf16,
+  // 131,000 tokens, 8 heads of 128: 79 us against 157; 512 segments of up to
+  // 600 tokens, 4 heads of 64: 79 against 80; with 33 to 60 rows a segment,
+  // the waves of siblings, 52 against 46).
+  const int rt = per_seg <= 8 ? 1 : per_seg <= 16 || per_seg > 24 ? 2 : 3;
   // One warp per unit when there are enough units to fill the device and the
   // page lists are short on average; else the CTA's warps share a unit.
   const int64_t avg = r.num_groups ? r.num_group_pages / r.num_groups : 0;
@@ -244,7 +251,7 @@ size_t attend_step_bytes(const imba_cache_desc& c, int32_t rows) {
   r.num_group_pages = INT32_MAX / IMBA_PAGE_TOKENS;
   r.num_q_heads = c.num_heads;
   size_t most = 0;
-  for (int rt : {1, 2, kTileGroups})
+  for (int rt : {1, 2, 3, kTileGroups})
     for (int warps : {1, kUnitWarps})
       most = std::max(most, attend_plan_view(c, r, shape_of(c, r, rt, warps, attend_step_most(rows)), nullptr).bytes);
   return most;

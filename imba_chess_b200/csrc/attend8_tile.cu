@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
       if (misc[2]) {
         __threadfence();
         if (tid == 0) *done = 0;
-        join_items<bf16, D>(a, it, head, lg, 0, kRows, tid, 2 * kRows);
+        join_items<bf16, D, 4>(a, it, head, lg, 0, kRows, tid, 2 * kRows);
       }
     }
     tc::fence_before_sync();

@@ -371,6 +371,51 @@ def test_attention_many_short_sequences():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("dqk,dv", [(32, 32), (64, 64), (32, 64), (64, 32), (96, 96), (128, 128)])
+def test_attention_tiles_of_24_rows(dqk, dv, dtype):
+    """Some 20 rows a segment with its shared heads: one tile each, of a
+    segment that sees nothing, of split and of short lists, with extra keys."""
+    rng = np.random.default_rng(dqk + 2 * dv)
+    lens, nrow, heads, share = [0, 30, 3000, 333, 17, 64], [5, 6, 5, 4, 5, 7], 2, 4
+    pool = _pool(heads=heads, dqk=dqk, dv=dv, pages=250)
+    page_off, pages, slots = _fill(pool, rng, lens + [50])
+    row_off = np.r_[0, np.cumsum(nrow)]
+    vis = np.concatenate([[max(0, n - r + 1 + i) if n % 2 else n for i in range(r)] for n, r in zip(lens, nrow)])
+    per = rng.integers(0, 4, len(vis))
+    off = np.r_[0, np.cumsum(per)]
+    slot = rng.choice(slots[sum(lens):], off[-1])
+    pos = vis + per
+    kpos = np.concatenate([vis[r] + np.arange(per[r]) for r in range(len(vis))])
+    q = _rand(rng, (len(vis), heads * share, dqk), dtype, 0.3)
+    bias = torch.tensor(rng.standard_normal((heads * share, 201)), dtype=torch.float32, device=DEV)
+    for more, extra in (({}, None), (dict(row_extra_off=off, extra_slot=slot, extra_pos=kpos), (off, slot, kpos))):
+        plan = paged.AttentionPlan(pool, row_off=row_off, row_vis=vis, page_off=page_off[:7], pages=pages,
+                                   num_q_heads=heads * share, positions=pos, **more)
+        for b in (None, bias):
+            for _ in range(2):  # the plan's counters are left as they were found
+                got = paged.paged_attention(pool, 0, plan, q, bias=b)
+            paged.check_status(pool)
+            _compare(got, _reference(pool, 0, q, dqk**-0.5, row_off, vis, page_off, pages,
+                                     None if b is None else _f64(b), pos, extra))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_attention_tiles_of_24_rows_a_warp_each(dtype):
+    rng = np.random.default_rng(24)
+    lens = rng.integers(0, 40, 600).tolist()
+    lens[5] = 1200
+    pool = _pool(heads=2, pages=sum(-(-n // 16) for n in lens) + 1)
+    page_off, pages, _ = _fill(pool, rng, lens)
+    row_off, vis = 5 * np.arange(601), np.repeat(lens, 5)
+    q = _rand(rng, (3000, 8, 64), dtype, 0.3)
+    plan = paged.AttentionPlan(pool, row_off=row_off, row_vis=vis, page_off=page_off, pages=pages, num_q_heads=8)
+    for _ in range(2):
+        got = paged.paged_attention(pool, 0, plan, q)
+    paged.check_status(pool)
+    _compare(got, _reference(pool, 0, q, 0.125, row_off, vis, page_off, pages))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("lens", [[0, 5, 40], [300, 900, 16]])
 def test_attention_extra_keys(lens, dtype):
     """Suffix chains and own tokens after the visible prefix, rows without
