@@ -14,9 +14,11 @@
 // blocks' scales multiply scores and weights, not elements.  The cache is the
 // 16-row operand, S' = K Q' and O' = V' P', so that a tile is eight query rows
 // and not sixteen: a decode step has few of them, and every instruction but
-// the conversions is per row.  (With the rows as the 16-row operand a step of
-// 1,024 one-token games took 45 us, 32 long sequences 324.)  The weights pass
-// from the result's layout to the operand's by movmatrix.
+// the conversions is per row.  The weights pass from the result's layout to the
+// operand's by movmatrix.  A step of 1,024 one-token games (8 heads of 64)
+// takes 35 us, 1.7 TB/s, of which the chain of dependent loads and the plan
+// are the most; 32 long sequences (8 heads of 128, four query heads each)
+// 260 us, 5.0 TB/s.  With the rows as the 16-row operand they took 45 and 324.
 //
 // A contraction may run over its dimension in any order as long as both
 // operands agree, so the order is chosen for the loads: a lane reads 16 (8
@@ -725,7 +727,10 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
 template <typename T, int DQK, int DV, int RT, int NW>
 cudaError_t launch_one(const AttendArgs& a, cudaStream_t s) {
   using D = Dims<DQK, DV, RT>;
-  constexpr int kCtas = attend8_ctas(DQK, RT), kStages = 3;
+  constexpr int kCtas = attend8_ctas(DQK, RT);
+  // Two pages of each warp in flight behind the one at work: with three (and a
+  // CTA less an SM at head size 128) the long sequences took 292 us, not 264.
+  constexpr int kStages = 3;
   constexpr size_t ring = (size_t)kUnitWarps * kStages * D::STAGE;
   constexpr size_t smem = NW > 1 && D::MERGE > ring ? D::MERGE : ring;
   auto fn = attend8_kernel<T, DQK, DV, RT, NW, kStages, kCtas>;

@@ -198,7 +198,11 @@ namespace {
 
 // Rows a segment (with its shared heads) from which the tcgen05 kernel's tiles
 // of 128 are better than tiles of 16 by mma.sync.
-constexpr int64_t kTileFrom = 64;
+// (8 heads of 64, segments of 2k to 12k tokens: 64 rows 99 us against 91, 96
+// rows 107 against 119, 256 rows 160 against 248; heads of 128: 64 rows 180
+// against 139, 96 rows 196 against 191, 256 rows 300 against 422; segments of
+// up to 600 tokens turn at the same numbers of rows.)
+constexpr int64_t kTileFrom = 80;
 
 // The shape with tiles of 8 rt rows and `warps` warps a unit.
 AttendShape shape_of(const imba_cache_desc& c, const imba_attend_desc& r, int rt, int warps, int64_t most) {
@@ -213,7 +217,9 @@ AttendShape shape_of(const imba_cache_desc& c, const imba_attend_desc& r, int rt
   sh.min_pages = warps == 1 ? 16 : 8;
   // About four CTAs' worth of units for each that is resident (two of the
   // tcgen05 kernel's, whose parts are large), but fewer for a step of few
-  // tiles, so that one is not joined from more than about 32 parts.
+  // tiles, so that one is not joined from more than about 32 parts: one
+  // sequence of 131,000 tokens (20 rows, 8 heads of 128) takes 79 us as one
+  // wave and 131 as four, 32 long sequences 318 and 260.
   const int ctas = std::min(attend8_ctas(c.attention_dim, rt), 2);
   const int64_t few = std::max<int64_t>((flat + sh.tile_rows - 1) / sh.tile_rows, r.num_segs) * c.num_heads * 32;
   const int waves = (int)std::min<int64_t>(rt == kTileGroups ? 2 : 4, std::max<int64_t>(1, few / (148 * ctas)));
@@ -229,7 +235,9 @@ AttendShape shape_of(const imba_cache_desc& c, const imba_attend_desc& r, int rt
 
 AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r, int64_t most) {
   const int64_t flat = (int64_t)r.num_rows * (r.num_q_heads / c.num_heads);
-  // Rows of a tile by what a segment has on average.
+  // Rows of a tile by what a segment has on average: the fewest groups that
+  // hold it (the games' step, one row a segment: 44 us with one group, 48 with
+  // two; waves of siblings: 54 with one, 43 with two).
   const int64_t per_seg = r.num_segs ? (flat + r.num_segs - 1) / r.num_segs : 0;
   if (r.num_extra == 0 && c.attention_dim == c.linear_dim && c.attention_dim % 64 == 0 && per_seg >= kTileFrom)
     return shape_of(c, r, kTileGroups, kUnitWarps, most);
@@ -240,6 +248,8 @@ AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r, in
   const int rt = per_seg <= 8 ? 1 : per_seg <= 16 || per_seg > 24 ? 2 : 3;
   // One warp per unit when there are enough units to fill the device and the
   // page lists are short on average; else the CTA's warps share a unit.
+  // (1,024 one-token games of up to 300 tokens: 44 us against 90; the waves of
+  // siblings 52 against 145.)
   const int64_t avg = r.num_groups ? r.num_group_pages / r.num_groups : 0;
   const int64_t busy = std::max<int64_t>(flat / (kTileRows * rt), r.num_segs) * c.num_heads;
   return shape_of(c, r, rt, busy >= 148 * 8 && avg <= 32 ? 1 : kUnitWarps, most);

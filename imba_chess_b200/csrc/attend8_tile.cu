@@ -9,17 +9,19 @@
 // shared memory (K by rows of dimensions, V by rows of a token's dimensions,
 // an MN-major operand; both with the 128-byte swizzle), one block ahead of the
 // products; eight warps are the tile's rows, two threads a row, each with half
-// of a block's keys (one thread a row and all 64 keys left the SM waiting for
-// its instructions: 215 us against 145 for 4 x 512 rows of 16 heads over 2k to
-// 8k tokens): they read S from TMEM, agree on the row's maximum, weigh and
-// write P; a lane of the last page warp issues the
-// products: P V of a block, S of the block after next (whose tiles are ready:
-// three stages), and then turns its page of the block that P V makes room for.  Scales stay out of the products: K's
-// multiplies a page's scores, V's is in its weights' exponent.
+// of a block's keys: they read S from TMEM, agree on the row's maximum, weigh
+// and write P; a lane of the last page warp issues the products: P V of a
+// block, S of the block after next (whose tiles are ready: three stages), and
+// its warp then turns its page of the block that P V makes room for.  Scales
+// stay out of the products: K's multiplies a page's scores, V's is in its
+// weights' exponent.
 //
-// What bounds it: the exponentials and the few instructions a score takes
-// besides (16 MUFU lanes an SM and cycle), so two CTAs share an SM and each
-// has 64-key blocks: 256 TMEM columns, 80 KB (head size 64).
+// What bounds it: the chain of a block, S to maxima to weights to P to P V
+// (some 4,000 cycles a block of a CTA), so two CTAs share an SM (64-key blocks, 256 TMEM columns, 82 KB at head size 64).
+// 4 x 512 rows of 16 heads of 64 over 2k to 8k tokens take 179 us, 0.2 PFLOP/s;
+// with one thread a row and all 64 keys 215, two stages of K and V 205, a
+// fourth page warp apart from the products' lane 194, and tiles of 16 rows by
+// mma.sync 280.
 //
 // Numerics as in the mma.sync kernel (attend8_kernel.cuh).  V's scales of a
 // block's four pages are held against one reference; where they lie more than

@@ -19,6 +19,12 @@
 //  - sparse (decode steps: one new token in most pages): two warps take a
 //    page, lanes are (head, eight elements), and nothing waits for the CTA.
 // Queries do not go to a page: a warp turns a row, in row order.
+//
+// What bounds it: for documents the bytes (1.2 GB of four documents, 8 heads of
+// 128 and 32 query heads, in 254 us, 4.8 TB/s; the rotation and the codes hide
+// behind the loads of the next block), for prefixes of many games the pages'
+// turns and codes as well (57k tokens of 8 heads of 64, 85 us, 3.1 TB/s), for a
+// decode step the launch (1,024 tokens 4.4 us, one token 2.8).
 #pragma once
 
 #include <algorithm>
@@ -941,7 +947,9 @@ imba_status_t launch_append(const imba_cache_desc& c, const imba_pool_desc& pool
   const int64_t q_blocks = a.Hq ? (d.num_rows + kWarps * a.q_rows - 1) / (kWarps * a.q_rows) : 0;
   cudaError_t e = cudaErrorInvalidValue;
   if (c.dtype == IMBA_DTYPE_E4M3) {
-    // a page a CTA with two tokens or more in it on average, else kSparse;
+    // A page a CTA with two tokens or more in it on average, else kSparse
+    // (1,024 games' tokens, one a page: 12.2 us by CTA, 4.3 by warps; 1,024
+    // prefixes of up to 300 tokens 85 and 89, four documents 253 and 249);
     // as many CTAs as there is room for, which go from page to page
     const int ctas = append_ctas(sizeof(T), std::max(c.attention_dim, c.linear_dim));
     a.page_blocks = (int)std::min<int64_t>((d.num_rows + 1) / 2, 148 * ctas);
