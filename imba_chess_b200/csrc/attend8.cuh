@@ -22,6 +22,12 @@ constexpr int attend8_ctas(int dqk, int rt) {
   return rt == kTileGroups ? 2 : dqk > 64 ? (rt == 1 ? 2 : 1) : rt == 1 ? 3 : rt == 2 || dqk == 32 ? 2 : 1;
 }
 
+// Bounds that keep a bias column, key - position + max_pos - 1, within 32 bits:
+// the pages of a step's lists (2^30 tokens), and the largest max_pos.  A
+// position below -kMostPos puts every key into the last column, as it does.
+constexpr int kMostPages = 1 << 26;
+constexpr int kMostPos = 1 << 28;
+
 struct AttendRow {  // one flattened row of a tile
   int row;          // -1: none
   int vis;          // visible tokens of the page list

@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
           const int k = e >> 1;
           s[r][e] *= ks[k] * st.fac[r][e & 1];
           if (biased)
-            s[r][e] += take_bias(__ldg(st.bias[r][e & 1] + min(max(kpos[k] + st.pos[r][e & 1], 0), last)));
+            s[r][e] += take_bias(__ldg(st.bias[r][e & 1] + min(max((int64_t)kpos[k] + st.pos[r][e & 1], (int64_t)0), (int64_t)last)));
           if (kslot[k] < 0 || kown[k] != 8 * r + 2 * t + (e & 1)) s[r][e] = -INFINITY;
         }
       st.weigh(s, 0.f, 1.f);

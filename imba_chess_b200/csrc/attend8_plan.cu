@@ -184,7 +184,7 @@ __global__ void attend_rows_kernel(imba_attend_desc r, AttendShape sh, AttendPla
       o.row = row_at(r, b.x + f / sh.share);
       if (o.row >= 0) {
         o.vis = visible(r, o.row, b.z * IMBA_PAGE_TOKENS);
-        o.pos = r.positions ? r.positions[o.row] : 0;
+        o.pos = r.positions ? max(r.positions[o.row], -kMostPos) : 0;
         o.head = f % sh.share;
       }
     }
@@ -258,7 +258,7 @@ AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r, in
 size_t attend_step_bytes(const imba_cache_desc& c, int32_t rows) {
   imba_attend_desc r = {};
   r.num_rows = r.num_segs = r.num_groups = rows;  // every chunk holds a row
-  r.num_group_pages = INT32_MAX / IMBA_PAGE_TOKENS;
+  r.num_group_pages = kMostPages;
   r.num_q_heads = c.num_heads;
   size_t most = 0;
   for (int rt : {1, 2, 3, kTileGroups})
@@ -306,7 +306,7 @@ imba_status_t validate_rows(const imba_cache_desc* c, const imba_attend_desc* r)
   if (!r || r->num_rows < 0 || r->num_segs < 0 || r->num_groups < 0 || r->num_group_pages < 0 || r->num_extra < 0)
     return IMBA_ERR_ARG;
   if (r->num_q_heads <= 0 || r->num_q_heads % c->num_heads) return IMBA_ERR_ARG;
-  if (r->num_group_pages > INT32_MAX / IMBA_PAGE_TOKENS) return IMBA_ERR_RANGE;
+  if (r->num_group_pages > kMostPages) return IMBA_ERR_RANGE;
   if ((int64_t)r->num_rows * (r->num_q_heads / c->num_heads) > (1 << 28) || r->num_segs > (1 << 28))
     return IMBA_ERR_UNSUPPORTED;
   if (!r->seg_group && r->num_segs > r->num_groups) return IMBA_ERR_ARG;
@@ -357,6 +357,7 @@ imba_status_t imba_attend(const imba_cache_desc* cache, const imba_pool_desc* po
   if (!args) return IMBA_ERR_ARG;
   if (args->layer < 0 || args->layer >= cache->num_layers) return IMBA_ERR_RANGE;
   if (args->dtype != IMBA_DTYPE_F32 && args->dtype != IMBA_DTYPE_BF16) return IMBA_ERR_ARG;
+  if (args->bias && args->max_pos > imba::kMostPos) return IMBA_ERR_UNSUPPORTED;
   if (rows->num_rows == 0 || rows->num_segs == 0) return IMBA_OK;
   if (!args->q || !args->out) return IMBA_ERR_ARG;
   if (args->bias && (args->max_pos <= 0 || !rows->positions)) return IMBA_ERR_ARG;

@@ -384,7 +384,7 @@ typedef struct imba_attend_desc {
   int32_t num_rows;
   int32_t num_segs;
   int32_t num_groups;
-  int32_t num_group_pages;
+  int32_t num_group_pages;          /* at most 2^26                                  */
   int32_t num_extra;
   int32_t num_q_heads;              /* a multiple of the cache's heads               */
   const int32_t* seg_group;         /* [S], or NULL: segment s is of group s         */
@@ -392,7 +392,8 @@ typedef struct imba_attend_desc {
   const int32_t* seg_nrows;         /* [S] or NULL                                   */
   const int32_t* row_perm;          /* [R] or NULL: row i of the segments' row order */
   const int32_t* row_vis;           /* [R]                                           */
-  const int32_t* positions;         /* [R] or NULL (the bias needs them)             */
+  const int32_t* positions;         /* [R] or NULL (the bias needs them); one below  */
+                                    /* -2^28 counts as -2^28                         */
   const int32_t* group_page_off;    /* [G + 1]                                       */
   const int32_t* group_pages;
   const int32_t* row_extra_off;     /* [R + 1] or NULL                               */
@@ -416,7 +417,7 @@ typedef struct imba_attend_args {
   int64_t q_stride[2];          /* (row, head), elements                                    */
   int64_t out_stride[2];
   float scale;                  /* of q . k                                                 */
-  int32_t max_pos;              /* bias has 2 max_pos - 1 columns                           */
+  int32_t max_pos;              /* bias has 2 max_pos - 1 columns; at most 2^28             */
   const float* bias;            /* [num_q_heads, 2 max_pos - 1] or NULL: column             */
                                 /* clamp(key position - positions[r] + max_pos - 1)         */
 } imba_attend_args;

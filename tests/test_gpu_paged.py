@@ -504,6 +504,32 @@ def test_attention_not_finite_queries_stay_in_their_rows():
         assert torch.equal(got[r, h], good[r, h])
 
 
+@pytest.mark.parametrize("rows", [7, 100])
+def test_attention_bias_at_extreme_positions(rows):
+    """Positions at both ends of int32: every key is far before or behind,
+    and the columns are the table's first and last."""
+    rng = np.random.default_rng(rows)
+    big = 2**31 - 1
+    pool = _pool(heads=1, pages=20)
+    page_off, pages, slots = _fill(pool, rng, [150, 20])
+    row_off, vis = np.array([0, rows]), np.full(rows, 150)
+    pos = rng.choice([-big - 1, -big, -(2**30), -1, 0, 75, 2**30, big - 100, big - 1, big], rows)
+    pos[:4] = -big - 1, big, big - 4, 60
+    q = _rand(rng, (rows, 1, 64), torch.bfloat16, 0.3)
+    bias = torch.tensor(rng.standard_normal((1, 21)), dtype=torch.float32, device=DEV)
+    plan = paged.AttentionPlan(pool, row_off=row_off, row_vis=vis, page_off=page_off[:2], pages=pages[:10], num_q_heads=1, positions=pos)
+    got = paged.paged_attention(pool, 0, plan, q, bias=bias)
+    paged.check_status(pool)
+    _compare(got, _reference(pool, 0, q, 0.125, row_off, vis, page_off, pages, _f64(bias), pos))
+    off, slot = 2 * np.arange(rows + 1), rng.choice(slots[150:], 2 * rows)
+    kpos = np.where(np.repeat(pos, 2) > 0, np.repeat(pos, 2) - rng.integers(0, 9, 2 * rows), rng.choice([0, 3, big], 2 * rows))
+    plan = paged.AttentionPlan(pool, row_off=row_off, row_vis=vis, page_off=page_off[:2], pages=pages[:10], num_q_heads=1,
+                               positions=pos, row_extra_off=off, extra_slot=slot, extra_pos=kpos)
+    got = paged.paged_attention(pool, 0, plan, q, bias=bias)
+    paged.check_status(pool)
+    _compare(got, _reference(pool, 0, q, 0.125, row_off, vis, page_off, pages, _f64(bias), pos, (off, slot, kpos)))
+
+
 def test_attention_strides_and_rows_left_alone():
     """Strided queries and outputs; rows behind the last sequence keep what
     they held."""

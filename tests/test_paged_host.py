@@ -176,6 +176,20 @@ def test_library_refuses_malformed_calls(lib):
     assert lib.imba_attend_plan_bytes(byref(cache), byref(_native.AttendDesc(4, 2, 2, 8, 0, 6))) == 0
 
 
+def test_library_refuses_sizes_past_32_bit_columns(lib):
+    """Lists of more than 2^26 pages, and tables of more than 2^28 positions a side."""
+    byref = ctypes.byref
+    cache, pool, at = _native.CacheDesc(2, 4, 64, 64, _native.DTYPE_E4M3), _native.PoolDesc(1 << 20, 4), 1 << 20
+    rows = _native.AttendDesc(4, 2, 2, 1 << 26, 0, 4)
+    assert lib.imba_attend_plan_bytes(byref(cache), byref(rows)) > 0
+    more = _native.AttendDesc(4, 2, 2, (1 << 26) + 1, 0, 4)
+    assert lib.imba_attend_plan_bytes(byref(cache), byref(more)) == 0
+    for name in ("seg_row_off", "row_vis", "group_page_off", "group_pages", "positions"):
+        setattr(rows, name, at)
+    args = _native.AttendArgs(layer=0, dtype=_native.DTYPE_BF16, q=at, out=at, scale=1.0, max_pos=(1 << 28) + 1, bias=at)
+    assert lib.imba_attend(byref(cache), byref(pool), byref(rows), byref(args), at, 1 << 40, None) == _native.IMBA_ERR_UNSUPPORTED
+
+
 def test_cache_struct_layouts_match_c(tmp_path):
     gxx = shutil.which("g++")
     if gxx is None:
