@@ -21,7 +21,9 @@ written to ``pool``'s status word and raised by ``check_status(pool)``.
 
 A plan keeps the tensors it was made from and its scratch: calls on one plan
 must not overlap (two streams, two captured graphs), and the plan's tensors
-hold the step's rows as they were when it was made.
+hold the step's rows as they were when it was made.  A call on another stream
+than the plan's waits for nothing by itself, as with any tensor, and marks the
+plan's memory as used there; a captured graph needs its plans kept alive.
 """
 
 from __future__ import annotations
@@ -77,11 +79,13 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _call(pool: KVPool, what: str, *args) -> None:
+def _call(pool: KVPool, what: str, *args, plan=None) -> None:
     """One library call on the current stream of the pool's device."""
     index = pool.data.get_device()
     fn = _FNS.get(what) or _FNS.setdefault(what, getattr(_native.load(), what))
     stream = _raw_stream(index)
+    if plan is not None and stream != plan._stream:
+        _used_on(plan, index)
     if torch.cuda.current_device() == index:
         code = fn(*args, stream)
     else:
@@ -89,6 +93,16 @@ def _call(pool: KVPool, what: str, *args) -> None:
             code = fn(*args, stream)
     if code:
         _native.check(code, what)
+
+
+def _used_on(plan, index: int) -> None:
+    """The plan's memory is not handed out again before the current stream,
+    which is not the one that it was made on, has passed this call."""
+    with torch.cuda.device(index):
+        if not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream()
+            for t in plan._memory:
+                t.record_stream(stream)
 
 
 def _ints(x, pool: KVPool, what: str, shape: tuple[int, ...] | None = None) -> torch.Tensor:
@@ -166,6 +180,8 @@ class AppendPlan:
         self._desc = ctypes.create_string_buffer(_APPEND.size)
         self._refs = (ctypes.cast(self._desc, ctypes.POINTER(_native.AppendDesc)), self._plan.data_ptr(), need,
                       self.slots.data_ptr(), status.data_ptr())
+        self._memory = (self._plan, self.slots, status)
+        self._stream = _raw_stream(self._plan.get_device())
         _call(pool, "imba_append_plan", desc, self.num_rows, self.slots.data_ptr(), self._plan.data_ptr(), need,
               status.data_ptr())
 
@@ -221,7 +237,7 @@ def kv_append(pool: KVPool, layer: int, plan: AppendPlan, k: torch.Tensor, v: to
     ref, ptr, size, slots, status = plan._refs
     _APPEND.pack_into(plan._desc, 0, n, layer, _DTYPES[dtype], q_heads, slots, k.data_ptr(), v.data_ptr(), *q_ptrs,
                       *k.stride(), *v.stride(), *q_strides, *turns, status)
-    _call(pool, "imba_kv_append", cache, desc, ref, ptr, size)
+    _call(pool, "imba_kv_append", cache, desc, ref, ptr, size, plan=plan)
     return q_out
 
 
@@ -291,6 +307,8 @@ class AttentionPlan:
         self._args = ctypes.create_string_buffer(_ATTEND.size)
         self._refs = (ctypes.byref(d), ctypes.cast(self._args, ctypes.POINTER(_native.AttendArgs)),
                       self._plan.data_ptr(), need)
+        self._memory = (self._plan, status, *keep.values())
+        self._stream = _raw_stream(self._plan.get_device())
         _call(pool, "imba_attend_plan", cache, desc, ctypes.byref(d), self._plan.data_ptr(), need)
 
 
@@ -327,5 +345,5 @@ def paged_attention(pool: KVPool, layer: int, plan: AttentionPlan, q: torch.Tens
     (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
     _ATTEND.pack_into(plan._args, 0, layer, _DTYPES[dtype], q.data_ptr(), out.data_ptr(), q0, q1, o0, o1,
                       pool.attention_dim**-0.5 if scale is None else scale, max_pos, column)
-    _call(pool, "imba_attend", cache, desc, rows, args, ptr, size)
+    _call(pool, "imba_attend", cache, desc, rows, args, ptr, size, plan=plan)
     return out

@@ -759,6 +759,55 @@ def test_operators_together_under_a_graph():
     assert np.abs(_f64(eager[2][:1]) - ref[0]).max() <= 0.05 * np.abs(ref[0]).max()
 
 
+def test_plans_on_another_stream_keep_their_memory():
+    """A plan that is dropped while another stream still runs on it."""
+    pool = _pool()
+    rng = np.random.default_rng(53)
+    k, v, q = (_rand(rng, (4, h, 64)) for h in (2, 2, 2))
+    stream = torch.cuda.Stream()
+    rows = paged.AppendPlan(pool, [0, 1, 2, 3])
+    sees = paged.AttentionPlan(pool, row_off=[0, 4], row_vis=[1, 2, 3, 4], page_off=[0, 1], pages=[0], num_q_heads=2)
+    held = [(len(p._plan), p._plan.data_ptr()) for p in (rows, sees)]
+    paged.kv_append(pool, 0, rows, k, v)
+    want = paged.paged_attention(pool, 0, sees, q)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(100_000_000)
+        paged.kv_append(pool, 0, rows, k, v)
+        got = paged.paged_attention(pool, 0, sees, q)
+    del rows, sees
+    fresh = [torch.full((n,), 255, dtype=torch.uint8, device=DEV) for n, _ in held for _ in range(4)]
+    assert not {t.data_ptr() for t in fresh} & {at for _, at in held}
+    torch.cuda.synchronize()
+    paged.check_status(pool)
+    assert torch.equal(got, want)
+
+
+def test_pool_past_32_bits():
+    """Pages whose bytes lie past 2^32, in the last layer."""
+    rng = np.random.default_rng(59)
+    pool = _pool(layers=16, heads=8, pages=17000)  # 4.5 GB
+    assert pool.page_bytes * 16900 > 2**32
+    ids = np.array([16999, 3, 16990, 16500, 16998])
+    slots = (ids[:, None] * 16 + np.arange(16)).reshape(-1)[:75]
+    k, v = (_rand(rng, (75, 8, 64)) for _ in range(2))
+    paged.kv_append(pool, 15, paged.AppendPlan(pool, slots), k, v)
+    paged.check_status(pool)
+    got = paged.kv_read(pool, 15, slots, torch.float32)
+    for mine, want in zip(got, (k, v)):  # half a step of e4m3, at least that of the block's smallest codes
+        assert (np.abs(_f64(mine) - _f64(want)) <= np.maximum(2.0**-4 * np.abs(_f64(want)), 2.0**-10 * 2 * np.abs(_f64(want)).max() / 448)).all()
+    for rows in (1, 90):
+        q = _rand(rng, (rows, 8, 64), torch.bfloat16, 0.3)
+        row_off, vis = np.array([0, rows]), np.full(rows, 75)
+        plan = paged.AttentionPlan(pool, row_off=row_off, row_vis=vis, page_off=[0, 5], pages=ids, num_q_heads=8)
+        out = paged.paged_attention(pool, 15, plan, q)
+        paged.check_status(pool)
+        _compare(out, _reference(pool, 15, q, 0.125, row_off, vis, [0, 5], ids))
+    low = paged.kv_read(pool, 15, np.arange(48, 64), torch.float32)  # page 3 holds its own tokens
+    assert torch.equal(low[0], got[0][16:32])
+    assert not paged.kv_read(pool, 14, slots, torch.float32)[0].any()
+
+
 def test_refusals():
     pool, full = _pool(), _pool(torch.bfloat16)
     rng = np.random.default_rng(41)
