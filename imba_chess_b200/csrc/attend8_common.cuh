@@ -25,7 +25,12 @@ __device__ __forceinline__ float2 unpack_h2(uint32_t u) { return __half22float2(
 // kFar, a power of two, whose product with lg is exact: a row whose every key
 // carries the type's lowest value still weighs its keys by nothing else.
 constexpr float kFar = -1.2676506002282294e30f;  // -2^100
-__device__ __forceinline__ float take_bias(float b) { return b == -INFINITY ? b : fmaxf(b, kFar); }
+// A NaN stays one and makes its row NaN.
+__device__ __forceinline__ float take_bias(float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(b), "f"(kFar));
+  return b == -INFINITY ? b : r;
+}
 
 // exp of a difference of running maxima; 0 for a part that has seen nothing.
 __device__ __forceinline__ float weight_of(float a, float b, float lg) {

@@ -530,6 +530,34 @@ def test_attention_bias_at_extreme_positions(rows):
     _compare(got, _reference(pool, 0, q, 0.125, row_off, vis, page_off, pages, _f64(bias), pos, (off, slot, kpos)))
 
 
+@pytest.mark.parametrize("rows", [6, 20, 100])
+def test_attention_bias_not_a_number(rows):
+    """A NaN in the bias makes the rows NaN that see its key, and no others;
+    behind what a row sees it does nothing."""
+    rng = np.random.default_rng(rows)
+    n = 150
+    pool = _pool(heads=1, pages=20)
+    page_off, pages, _ = _fill(pool, rng, [n])
+    row_off, vis, pos = np.array([0, rows]), rng.integers(0, n + 1, rows), np.arange(rows)
+    q = _rand(rng, (rows, 2, 64), torch.bfloat16, 0.3)
+    table = rng.standard_normal((2, 2 * 256 - 1))
+    odd = table.copy()
+    column = 60 + 255
+    odd[1, column] = math.nan
+    plan = paged.AttentionPlan(pool, row_off=row_off, row_vis=vis, page_off=page_off, pages=pages, num_q_heads=2, positions=pos)
+    got = paged.paged_attention(pool, 0, plan, q, bias=torch.tensor(odd, dtype=torch.float32, device=DEV))
+    paged.check_status(pool)
+    sees = torch.tensor(vis > pos + 60, device=DEV)
+    assert sees.any() and not sees.all()
+    assert torch.isnan(got[sees, 1]).all()
+    bias = torch.tensor(table, dtype=torch.float32, device=DEV)
+    want, tol = _reference(pool, 0, q, 0.125, row_off, vis, page_off, pages, _f64(bias), pos)
+    hit = sees.cpu().numpy()
+    assert np.isfinite(_f64(got)[:, 0]).all() and np.isfinite(_f64(got)[~hit]).all()
+    off = np.abs(_f64(got) - want)
+    assert (off[:, 0] <= tol[:, 0]).all() and (off[~hit] <= tol[~hit]).all()
+
+
 def test_attention_strides_and_rows_left_alone():
     """Strided queries and outputs; rows behind the last sequence keep what
     they held."""
