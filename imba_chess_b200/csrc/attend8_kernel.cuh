@@ -51,6 +51,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ int add_sat(int a, int b) {
+  int r;
+  asm("add.sat.s32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // An 8 x 8 matrix of f16 from a fragment of its rows to one of its columns.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -546,7 +552,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
           const int k = e >> 1;
           s[r][e] *= ks[k] * st.fac[r][e & 1];
           if (biased)
-            s[r][e] += take_bias(__ldg(st.bias[r][e & 1] + min(max((int64_t)kpos[k] + st.pos[r][e & 1], (int64_t)0), (int64_t)last)));
+            s[r][e] += take_bias(__ldg(st.bias[r][e & 1] + min(max(add_sat(kpos[k], st.pos[r][e & 1]), 0), last)));
           if (kslot[k] < 0 || kown[k] != 8 * r + 2 * t + (e & 1)) s[r][e] = -INFINITY;
         }
       st.weigh(s, 0.f, 1.f);
