@@ -17,9 +17,9 @@ constexpr int kTileGroups = 16;  // rt of the tcgen05 kernel's tiles of 128 rows
 
 // CTAs an SM, by what a lane's rows take in registers (four of 64 registers
 // for one group of rows: 42 us against 36 with three of 80 for 1,024 games).
-// For the tcgen05 kernel, what a plan counts with.
+// The tcgen05 kernel's are what shared memory holds.
 constexpr int attend8_ctas(int dqk, int rt) {
-  return rt == kTileGroups ? 2 : dqk > 64 ? (rt == 1 ? 2 : 1) : rt == 1 ? 3 : rt == 2 || dqk == 32 ? 2 : 1;
+  return rt == kTileGroups ? (dqk > 64 ? 1 : 2) : dqk > 64 ? (rt == 1 ? 2 : 1) : rt == 1 ? 3 : rt == 2 || dqk == 32 ? 2 : 1;
 }
 
 // Bounds that keep a bias column, key - position + max_pos - 1, within 32 bits:
@@ -55,6 +55,7 @@ struct AttendShape {
   int max_parts;
   int min_pages;    // pages of a split item, at least
   int target;       // items that splitting aims at
+  int waves;        // how many times the resident CTAs that is
 };
 
 // Plan memory, in this order, each part aligned to 256 bytes.

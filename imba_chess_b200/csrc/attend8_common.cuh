@@ -74,7 +74,8 @@ __device__ __forceinline__ void out_store4(T* p, bool vec, const float (&x)[4]) 
 // Rows r0 .. r0 + n - 1 of a split tile joined over its items, by `nthr`
 // threads from tid on, kAhead parts in flight.  The last item's CTA joins alone
 // while others idle, so what it costs is latency: 74 parts of 24 rows of 128
-// took 140 us of a call with four in flight, 131 with eight.
+// made a call of 140 us with four in flight, of 131 with eight; the tcgen05
+// kernel, short of registers there, is 2 % slower with eight.
 template <typename T, int DV, int kAhead>
 __device__ __forceinline__ void join_items(const AttendArgs& a, const AttendItem& it, int head, float lg, int r0, int n,
                                            int tid, int nthr) {

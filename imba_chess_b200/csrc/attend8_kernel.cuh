@@ -18,7 +18,7 @@
 // operand's by movmatrix.  A step of 1,024 one-token games (8 heads of 64)
 // takes 35 us, 1.7 TB/s, of which the chain of dependent loads and the plan
 // are the most; 32 long sequences (8 heads of 128, four query heads each)
-// 260 us, 5.0 TB/s.  With the rows as the 16-row operand they took 45 and 324.
+// 263 us, 4.9 TB/s.  With the rows as the 16-row operand they took 45 and 324.
 //
 // A contraction may run over its dimension in any order as long as both
 // operands agree, so the order is chosen for the loads: a lane reads 16 (8

@@ -165,7 +165,11 @@ __global__ void __launch_bounds__(kPlanThreads) attend_items_kernel(imba_attend_
     if (t < ntiles) {
       a = p.tiles[2 * t];
       b = p.tiles[2 * t + 1];
-      n = max(1, min((a.w + per - 1) / per, most_parts(a.w, sh.rt)));
+      n = (a.w + per - 1) / per;
+      // a single wave is not passed by a few items (152 units on 148 SMs: 488 us
+      // against 313 for 256 rows, 4 heads of 128 and 131,000 tokens)
+      if (sh.waves == 1) n = min(n, (int)((unsigned long long)a.w * sh.target / max(total, 1ull)));
+      n = max(1, min(n, most_parts(a.w, sh.rt)));
     }
     const int at = nitems + block_scan(n, warp_sums, &sum);
     nitems += sum;
@@ -209,9 +213,9 @@ namespace {
 // Rows a segment (with its shared heads) from which the tcgen05 kernel's tiles
 // of 128 are better than tiles of 16 by mma.sync.
 // (8 heads of 64, segments of 2k to 12k tokens: 64 rows 99 us against 91, 96
-// rows 107 against 119, 256 rows 160 against 248; heads of 128: 64 rows 180
-// against 139, 96 rows 196 against 191, 256 rows 300 against 422; segments of
-// up to 600 tokens turn at the same numbers of rows.)
+// rows 98 against 119, 256 rows 160 against 248; heads of 128: 64 rows 180
+// against 139, 96 rows 181 against 191, 256 rows 283 against 422; segments of
+// up to 600 tokens turn at about the same numbers of rows.)
 constexpr int64_t kTileFrom = 80;
 
 // The shape with tiles of 8 rt rows and `warps` warps a unit.
@@ -228,11 +232,11 @@ AttendShape shape_of(const imba_cache_desc& c, const imba_attend_desc& r, int rt
   // About four CTAs' worth of units for each that is resident (two of the
   // tcgen05 kernel's, whose parts are large), but fewer for a step of few
   // tiles, so that one is not joined from more than about 32 parts: one
-  // sequence of 131,000 tokens (20 rows, 8 heads of 128) takes 79 us as one
+  // sequence of 131,000 tokens (20 rows, 8 heads of 128) takes 80 us as one
   // wave and 131 as four, 32 long sequences 318 and 260.
   const int ctas = std::min(attend8_ctas(c.attention_dim, rt), 2);
   const int64_t few = std::max<int64_t>((flat + sh.tile_rows - 1) / sh.tile_rows, r.num_segs) * c.num_heads * 32;
-  const int waves = (int)std::min<int64_t>(rt == kTileGroups ? 2 : 4, std::max<int64_t>(1, few / (148 * ctas)));
+  const int waves = sh.waves = (int)std::min<int64_t>(rt == kTileGroups ? 2 : 4, std::max<int64_t>(1, few / (148 * ctas)));
   sh.target = (int)std::min<int64_t>(most, std::max(1, 148 * ctas * waves * (kUnitWarps / warps) / c.num_heads));
   const int64_t by_len = (int64_t)sh.max_tiles * ((r.num_group_pages + sh.min_pages - 1) / sh.min_pages);
   const int64_t cut = std::min<int64_t>(by_len, sh.target);  // full-size items; each tile may add one smaller
