@@ -97,7 +97,7 @@ imba_status_t validate_pool(const imba_pool_desc* pool) {
 extern "C" {
 
 size_t imba_cache_pool_bytes(const imba_cache_desc* cache, int64_t num_pages) {
-  if (imba::validate_cache(cache) != IMBA_OK || num_pages <= 0) return 0;
+  if (imba::validate_cache(cache) != IMBA_OK || num_pages <= 0 || num_pages > INT32_MAX / IMBA_PAGE_TOKENS) return 0;
   const int64_t elems = imba::cache8_page_bytes(*cache);
   if (cache->dtype == IMBA_DTYPE_E4M3)
     return (size_t)((elems + (int64_t)cache->num_layers * 2 * cache->num_heads) * num_pages);

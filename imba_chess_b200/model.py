@@ -22,7 +22,9 @@ value logits are fp32; returned k/v are in the model dtype.
 With ``kv_dtype=torch.float8_e4m3fn`` the model's pools hold keys and values
 in 8 bits (``kvpool``), half of bf16: its steps round each block of 16 tokens
 and head to e4m3 with a power-of-two scale and attend over the codes
-(``paged``'s operators).  Weights and activations stay in ``dtype``.
+(``paged``'s operators).  Weights and activations stay in ``dtype``.  A token
+that raises its block's scale rounds the block's earlier ones once more, so a
+page's tokens depend, within that rounding, on what is appended to it later.
 """
 
 from __future__ import annotations

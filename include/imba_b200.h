@@ -318,13 +318,13 @@ typedef struct imba_cache_desc {
   int32_t dtype;            /* IMBA_DTYPE_*                                 */
 } imba_cache_desc;
 
-/* Bytes of a pool of num_pages pages (0: a geometry the operators do not
- * take).  The base is 256-byte aligned. */
+/* Bytes of a pool of num_pages pages (0: a geometry or a number of pages the
+ * operators do not take).  The base is 256-byte aligned. */
 IMBA_API size_t imba_cache_pool_bytes(const imba_cache_desc* cache, int64_t num_pages);
 
 /* The tokens of one step grouped by the page they go to, for
- * imba_kv_append on a pool in 8 bits: made once per step from the rows'
- * slots, used for every layer.  Row r goes to slot slots[r]; -1 is a padding
+ * imba_kv_append: made once per step from the rows' slots, used for every
+ * layer.  Row r goes to slot slots[r]; -1 is a padding
  * row, which is passed over; other slots outside the pool are skipped and
  * reported (IMBA_ERR_RANGE).  Of rows with the same slot the last one is
  * stored.  `plan` is device memory, 256-byte aligned. */
@@ -363,7 +363,7 @@ typedef struct imba_append_desc {
   imba_rotary_desc rotary;
   int32_t* status;
 } imba_append_desc;
-/* `plan` (of the same slots) is needed for a pool in 8 bits, else NULL. */
+/* `plan` is imba_append_plan's, of the same pool, rows and slots. */
 IMBA_API imba_status_t imba_kv_append(const imba_cache_desc* cache, const imba_pool_desc* pool,
                                       const imba_append_desc* append, const void* plan, size_t plan_bytes,
                                       void* stream);

@@ -177,9 +177,13 @@ def test_library_refuses_malformed_calls(lib):
 
 
 def test_library_refuses_sizes_past_32_bit_columns(lib):
-    """Lists of more than 2^26 pages, and tables of more than 2^28 positions a side."""
+    """Lists of more than 2^26 pages, and tables of more than 2^28 positions a side;
+    pools whose slots are no int32."""
     byref = ctypes.byref
     cache, pool, at = _native.CacheDesc(2, 4, 64, 64, _native.DTYPE_E4M3), _native.PoolDesc(1 << 20, 4), 1 << 20
+    most = (2**31 - 1) // 16
+    assert lib.imba_cache_pool_bytes(byref(cache), most) == most * 2 * 4 * (16 * 128 + 2)
+    assert lib.imba_cache_pool_bytes(byref(cache), most + 1) == 0 == lib.imba_cache_pool_bytes(byref(cache), 1 << 60)
     rows = _native.AttendDesc(4, 2, 2, 1 << 26, 0, 4)
     assert lib.imba_attend_plan_bytes(byref(cache), byref(rows)) > 0
     more = _native.AttendDesc(4, 2, 2, (1 << 26) + 1, 0, 4)
