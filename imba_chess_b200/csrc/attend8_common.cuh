@@ -21,21 +21,20 @@ __device__ __forceinline__ float2 unpack_h2(uint32_t u) { return __half22float2(
 
 // Scores are kept in log2 without a bias (the factor log2 e joins the
 // query's), with one as natural logarithms, where the bias is added as it is;
-// `lg` takes them to log2.  A bias below kFar that is not -inf counts as
-// kFar, a power of two, whose product with lg is exact: a row whose every key
-// carries the type's lowest value still weighs its keys by nothing else.
-constexpr float kFar = -1.2676506002282294e30f;  // -2^100
-// A NaN stays one and makes its row NaN.
-__device__ __forceinline__ float take_bias(float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(b), "f"(kFar));
-  return b == -INFINITY ? b : r;
-}
+// `lg` takes them to log2.  A weight is 2^(lg (score - maximum) + kShift), the
+// maximum subtracted first: that difference is exact where the weight matters.
+// (In one step, lg score + (kShift - lg maximum), the product would be rounded,
+// by 64 at a mask of -1e9, and its keys would get weights of 2^64 or none.)  So
+// keys that carry any mask, the type's lowest value too, weigh by their
+// differences alone.
+//
+// Running maxima start at the lowest finite value, so that the difference to a
+// key that is not seen (-inf) is -inf and not NaN; a row that has seen nothing
+// has no weight either, whatever its maximum.
+constexpr float kLowest = -3.4028234663852886e38f;
 
-// exp of a difference of running maxima; 0 for a part that has seen nothing.
-__device__ __forceinline__ float weight_of(float a, float b, float lg) {
-  return a == -INFINITY ? 0.f : exp2_approx((a - b) * lg);
-}
+// exp of a difference of running maxima.
+__device__ __forceinline__ float weight_of(float a, float b, float lg) { return exp2_approx((a - b) * lg); }
 
 // Four consecutive elements of a row as floats.
 template <typename T>
@@ -89,7 +88,7 @@ __device__ __forceinline__ void join_items(const AttendArgs& a, const AttendItem
     const int r = r0 + i / (DV / 4), e = i % (DV / 4) * 4;
     const AttendRow row = rows[r];
     if (row.row < 0) continue;
-    float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    float m = kLowest, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < it.splits; s0 += kAhead) {
       float2 ml[kAhead];
       float4 o[kAhead];

@@ -136,7 +136,6 @@ struct Rows {
   int vis[RT][2], pos[RT][2];    // visible tokens; the bias column of a key is its position plus pos, clamped
   const float* bias[RT][2];      // the row's bias (the call has one, or none of them is read)
   float m[RT][2], l[RT][2];      // running maximum, sum over this lane's keys
-  float ref[RT][2];              // kShift - lg m: a weight is 2^(lg score + ref)
   float lg, slack;               // from scores to log2; kSlack in scores
   float o[RT][D::MV][4];
   int vref, vmost;               // scale byte that O is held in units of, 0: none yet; the largest so far
@@ -151,7 +150,7 @@ struct Rows {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         mx[i][r] = fmaxf(s[i][r], s[i][2 + r]);
-        raise |= mx[i][r] > m[i][r] + slack;
+        raise |= mx[i][r] - m[i][r] > slack;
       }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -161,7 +160,6 @@ struct Rows {
           const float now = fmaxf(m[i][r], keys_max(mx[i][r]));
           const float w = weight_of(m[i][r], now, lg);
           m[i][r] = now;
-          ref[i][r] = now == -INFINITY ? 0.f : fmaf(-now, lg, kShift);
           l[i][r] *= w;
 #pragma unroll
           for (int j = 0; j < D::MV; ++j) {
@@ -174,9 +172,9 @@ struct Rows {
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float from = ref[i][r] + up;
-        s[i][r] = exp2_approx(fmaf(s[i][r], lg, from));
-        s[i][2 + r] = exp2_approx(fmaf(s[i][2 + r], lg, from));
+        // (never fused with the product that made the score: the maximum is of rounded scores)
+        s[i][r] = exp2_approx(fmaf(__fsub_rn(s[i][r], m[i][r]), lg, kShift + up));
+        s[i][2 + r] = exp2_approx(fmaf(__fsub_rn(s[i][2 + r], m[i][r]), lg, kShift + up));
         l[i][r] = fmaf(s[i][r] + s[i][2 + r], down, l[i][r]);
       }
   }
@@ -266,8 +264,8 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
       st.vis[i][r] = u.y;
       st.pos[i][r] = a.call.max_pos - 1 - u.z;
       st.bias[i][r] = a.call.bias + (int64_t)(head * a.shape.share + u.w) * (2 * a.call.max_pos - 1);
-      st.m[i][r] = -INFINITY;
-      st.l[i][r] = st.ref[i][r] = 0.f;
+      st.m[i][r] = kLowest;
+      st.l[i][r] = 0.f;
     }
 #pragma unroll
     for (int j = 0; j < D::MV; ++j) st.o[i][j][0] = st.o[i][j][1] = st.o[i][j][2] = st.o[i][j][3] = 0.f;
@@ -419,7 +417,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[r][e] += take_bias(add[r][e]);
+        for (int e = 0; e < 4; ++e) s[r][e] += add[r][e];
     }
     const int id = __shfl_sync(0xffffffffu, ids, i & 31);
     if (key0 + IMBA_PAGE_TOKENS > it.minvis || id < 0) {
@@ -552,7 +550,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
           const int k = e >> 1;
           s[r][e] *= ks[k] * st.fac[r][e & 1];
           if (biased)
-            s[r][e] += take_bias(__ldg(st.bias[r][e & 1] + min(max(add_sat(kpos[k], st.pos[r][e & 1]), 0), last)));
+            s[r][e] += __ldg(st.bias[r][e & 1] + min(max(add_sat(kpos[k], st.pos[r][e & 1]), 0), last));
           if (kslot[k] < 0 || kown[k] != 8 * r + 2 * t + (e & 1)) s[r][e] = -INFINITY;
         }
       st.weigh(s, 0.f, 1.f);
@@ -692,7 +690,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
       const int tr = i / (DV / 4), e = i % (DV / 4) * 4;
       const int4 row = __ldg(tile + tr);
       if (row.x < 0) continue;
-      float mm = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+      float mm = kLowest, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kUnitWarps; ++w) mm = fmaxf(mm, sml[w * D::ROWS + tr].x);
 #pragma unroll

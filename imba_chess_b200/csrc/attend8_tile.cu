@@ -23,7 +23,9 @@
 // fourth page warp apart from the products' lane 194, and tiles of 16 rows by
 // mma.sync 280.
 //
-// Numerics as in the mma.sync kernel (attend8_kernel.cuh).  V's scales of a
+// Numerics as in the mma.sync kernel (attend8_kernel.cuh), but that ordinary
+// scores without a bias become weights in one fused step, which the rounding of
+// kShift - maximum puts off by 2^-8 of a unit of log2 at most, all alike.  V's scales of a
 // block's four pages are held against one reference; where they lie more than
 // 2^kSpread apart, the block's P V is done page by page.
 #include <algorithm>
@@ -44,6 +46,7 @@ constexpr int kHalf = kKeys / 2;   // keys of a row thread
 constexpr uint32_t kCols = 256;    // TMEM columns: S at 0 and 64, O from 128
 constexpr int kStages = 3;         // blocks of K and V
 constexpr int kSpread = 12;        // with kVWindow on both sides
+constexpr float kNear = 65536.f;   // largest maximum of the fused step
 constexpr uint32_t kPanel = 128;   // bytes of a swizzled row: 64 f16
 constexpr uint32_t kKvPanel = kKeys * kPanel, kRowPanel = kRows * kPanel;
 
@@ -453,7 +456,7 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
     const float fac = reinterpret_cast<const float*>(sm + M::kFac)[trow];
 
     const uint32_t pt = tc::smem_u32(sm + M::kP) + trow * kPanel;
-    float m = -INFINITY, l = 0.f, ref = 0.f;
+    float m = kLowest, l = 0.f, ref = kShift;  // ref: kShift, the maximum to be subtracted apart, or with it
     float unit = 1.f;  // O's
     uint32_t pv = 0;   // P written
     bool ok = true;
@@ -524,7 +527,7 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             float y = x[16 * p + j] * f[p];
-            if (biased) y += take_bias(__ldg(bias + min(max(col0 + b * kKeys + 16 * p + j, 0), last)));
+            if (biased) y += __ldg(bias + min(max(col0 + b * kKeys + 16 * p + j, 0), last));
             y = 16 * p + j < n ? y : -INFINITY;
             x[16 * p + j] = y;
             mx = fmaxf(mx, y);
@@ -536,14 +539,22 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
       maxima[(s * 2 + half) * kRows + trow] = mx;
       pair_sync();
       mx = fmaxf(mx, maxima[(s * 2 + 1 - half) * kRows + trow]);
-      if (__any_sync(0xffffffffu, mx > m + slack) || turned != 1.f) {
+      if (__any_sync(0xffffffffu, mx - m > slack) || turned != 1.f) {
         const float now = fmaxf(m, mx), w = weight_of(m, now, lg);
         m = now;
-        ref = now == -INFINITY ? 0.f : fmaf(-now, lg, kShift);
+        ref = biased || !(fabsf(now) <= kNear) ? kShift : kShift - now;
         l *= w;
         if (!rescale(w * turned)) {
           ok = false;
           continue;
+        }
+      }
+      if (ref == kShift) {  // (scores rounded as the maximum was, which a fused product would not be)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[16 * p + j] = __fsub_rn(__fmul_rn(x[16 * p + j], f[p]), m);
+          f[p] = 1.f;
         }
       }
       // Weights, two pages of sixteen, as f16 pairs.
