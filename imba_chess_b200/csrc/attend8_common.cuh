@@ -12,6 +12,10 @@ namespace {
 constexpr float kShift = 5.f;
 constexpr float kSlack = 4.f;
 constexpr int kVWindow = 6;  // 2^(kShift + kSlack + kVWindow) = 2^15 is finite in f16
+// A V scale that is further below O's units enters as this one: the weights'
+// f16 are zero either way, and no weight that counts is lost in the row's sum,
+// which is of the scaled weights.
+constexpr int kVLeast = -40;
 
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);

@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
     // V's scale as its ratio to vref, in the weights' exponent.
     const int vb = sc >> 8;
     if ((uint32_t)(vb - st.vref + kVWindow) > 2 * kVWindow && vb) st.follow(vb);
-    const int up = vb ? max(vb - st.vref, -126) : 0;
+    const int up = vb ? max(vb - st.vref, kVLeast) : 0;
     st.weigh(s, (float)up, __uint_as_float((uint32_t)(127 - up) << 23));
     uint32_t pb[RT][NP][2];
     st.pack(s, pb);

@@ -155,7 +155,7 @@ struct Units {
 #pragma unroll
       for (int p = 0; p < kPages; ++p) {
         const int vb = sc[p] < 0 ? 0 : sc[p] >> 8;
-        const int up = vb ? min(max(vb - vref, -126), kVWindow) : 0;
+        const int up = vb ? min(max(vb - vref, kVLeast), kVWindow) : 0;
         o.up[p] = (float)up;
         o.down[p] = __uint_as_float((uint32_t)(127 - up) << 23);
       }

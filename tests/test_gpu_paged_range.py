@@ -133,3 +133,29 @@ def test_scores_of_any_size(shape, dtype):
                 want[i, h], mean[i, h] = w.mean(0), np.abs(w).mean(0)
         r += m
     _check(got, want, mean, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("rows", [1, 20, 100])
+def test_values_at_both_ends_of_the_range(rows, dtype):
+    """A page of sixteen with values of 2^110, the others with 2^-96: the small
+    ones' keys count in the row's sum all the same."""
+    seqs, heads, pages = 80, 16, 32  # lists short and many: a unit sees sixteen pages of a list at least
+    n = 16 * pages
+    pool = _pool(heads=heads, pages=seqs * pages)
+    ids = np.random.default_rng(rows).permutation(seqs * pages)
+    slots = (ids[:, None] * 16 + np.arange(16)).reshape(-1)
+    big = np.arange(n) // 16 % 16 == 4
+    k, v = (torch.zeros((len(slots), heads, 64), device=DEV) for _ in range(2))
+    k[:, :, 9] = torch.tensor(np.tile(big, seqs), dtype=torch.float32, device=DEV)[:, None]
+    v[:] = torch.tensor(np.where(np.tile(big, seqs), 2.0**110, 2.0**-96), dtype=torch.float32, device=DEV)[:, None, None]
+    paged.kv_append(pool, 0, paged.AppendPlan(pool, slots), k, v)
+    q = torch.zeros((seqs * rows, heads, 64), dtype=dtype, device=DEV)
+    q[:, :, 9] = 7.0
+    plan = paged.AttentionPlan(pool, row_off=np.arange(seqs + 1) * rows, row_vis=np.full(seqs * rows, n),
+                               page_off=np.arange(seqs + 1) * pages, pages=ids, num_q_heads=heads)
+    got = paged.paged_attention(pool, 0, plan, q, scale=1.0)
+    paged.check_status(pool)
+    w = np.where(big, math.exp(7.0), 1.0)
+    want = np.full((seqs * rows, heads, 64), 2.0**110 * w[big].sum() / w.sum())
+    _check(got, want, want, dtype)
