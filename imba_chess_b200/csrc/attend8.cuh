@@ -66,8 +66,8 @@ struct AttendPlan {
   AttendItem* items;
   AttendRow* rows;       // [max_tiles][tile_rows]
   int* done;             // [max_tiles][H][8] items of a split tile (or of a part of its rows) that have finished
-  float2* ml;            // [max_parts][H][tile_rows] running maximum and sum
-  float* o;              // [max_parts][H][tile_rows][d_v]
+  float2* ml;            // [max_parts][H][tile_rows] maximum and sum
+  float* o;              // [max_parts][H][tile_rows][d_v] averages
   size_t bytes;
 };
 

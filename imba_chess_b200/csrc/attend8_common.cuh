@@ -75,7 +75,9 @@ __device__ __forceinline__ void out_store4(T* p, bool vec, const float (&x)[4]) 
 }
 
 // Rows r0 .. r0 + n - 1 of a split tile joined over its items, by `nthr`
-// threads from tid on, kAhead parts in flight.  The last item's CTA joins alone
+// threads from tid on, kAhead parts in flight.  A part is a row's average over
+// its keys, with their maximum and sum, and so is what has been joined: sums of
+// values at the upper end of fp32 would run over.  The last item's CTA joins alone
 // while others idle, so what it costs is latency: 74 parts of 24 rows of 128
 // made a call of 140 us with four in flight, of 131 with eight; the tcgen05
 // kernel, short of registers there, is 2 % slower with eight.
@@ -105,20 +107,22 @@ __device__ __forceinline__ void join_items(const AttendArgs& a, const AttendItem
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) now = fmaxf(now, ml[j].x);
-      const float was = weight_of(m, now, lg);
-      l *= was;
-      x[0] *= was, x[1] *= was, x[2] *= was, x[3] *= was;
+      const float was = l * weight_of(m, now, lg);
+      l = was;
       m = now;
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const float w = s0 + j < it.splits ? weight_of(ml[j].x, m, lg) : 0.f;
-        l += w * ml[j].y;
+        ml[j].x = s0 + j < it.splits ? weight_of(ml[j].x, m, lg) * ml[j].y : 0.f;
+        l += ml[j].x;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l, f = was * inv;
+      x[0] *= f, x[1] *= f, x[2] *= f, x[3] *= f;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float w = ml[j].x * inv;
         x[0] += w * o[j].x, x[1] += w * o[j].y, x[2] += w * o[j].z, x[3] += w * o[j].w;
       }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] *= inv;
     out_store4(static_cast<T*>(a.call.out) + row.row * a.call.out_stride[0] +
                    (int64_t)(head * a.shape.share + row.head) * a.call.out_stride[1] + e,
                vec, x);

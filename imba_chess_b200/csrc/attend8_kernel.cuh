@@ -122,7 +122,7 @@ struct Dims {
   static constexpr int KS = DQK / 16, MV = DV / 16;                    // k-steps of a score, row tiles of O'
   static constexpr int ROWS = kTileRows * RT;
   static constexpr int STAGE = IMBA_PAGE_TOKENS * (DQK + DV);  // a warp's page
-  static constexpr int MERGE = kUnitWarps * ROWS * (DV * 4 + 8) + 16;
+  static constexpr int MERGE = kUnitWarps * (ROWS * (DV * 4 + 8) + 4) + 16;
 };
 
 // A warp's rows and what they have summed up: lane (g, t) = (lane / 4, lane %
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
     }
   }
 
-  // Out: true units, relative to each row's running maximum.
+  // Out: averages in true units.
   const float unit_v = st.vref ? scale_of(st.vref) : 1.f;
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
         const int tr = 8 * i + 2 * t + r;
         const int4 row = __ldg(tile + tr);
         if (row.x < 0) continue;
-        const float f = it.part >= 0 ? unit_v : st.l[i][r] == 0.f ? 0.f : unit_v / st.l[i][r];
+        const float f = st.l[i][r] == 0.f ? 0.f : unit_v / st.l[i][r];
         if (it.part >= 0 && g == 0) a.plan.ml[part + tr] = make_float2(st.m[i][r], st.l[i][r]);
         T* out = static_cast<T*>(a.call.out) + row.x * a.call.out_stride[0] +
                  (int64_t)(head * a.shape.share + row.w) * a.call.out_stride[1];
@@ -662,11 +662,13 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
     }
   } else {
     // The warps' parts meet in shared memory (over the ring, which is idle).
-    float* so = reinterpret_cast<float*>(smem);                              // [warps][rows][DV]
+    float* so = reinterpret_cast<float*>(smem);                               // [warps][rows][DV], each in its warp's units
     float2* sml = reinterpret_cast<float2*>(so + kUnitWarps * D::ROWS * DV);  // [warps][rows]
-    int* flag = reinterpret_cast<int*>(sml + kUnitWarps * D::ROWS);
+    float* sunit = reinterpret_cast<float*>(sml + kUnitWarps * D::ROWS);      // [warps]
+    int* flag = reinterpret_cast<int*>(sunit + kUnitWarps);
     cp_wait<0>();
     __syncthreads();
+    if (lane == 0) sunit[warp] = unit_v;
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -680,7 +682,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
 #pragma unroll
           for (int q = 0; q < D::VV / 8; ++q) {
             float x[4];
-            four(i, r, c, q, unit_v, x);
+            four(i, r, c, q, 1.f, x);
             *reinterpret_cast<float4*>(dst + dim(c, q)) = make_float4(x[0], x[1], x[2], x[3]);
           }
       }
@@ -690,24 +692,26 @@ __global__ void __launch_bounds__(kUnitWarps * 32, CTAS) attend8_kernel(AttendAr
       const int tr = i / (DV / 4), e = i % (DV / 4) * 4;
       const int4 row = __ldg(tile + tr);
       if (row.x < 0) continue;
-      float mm = kLowest, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+      float mm = kLowest, l = 0.f, f[kUnitWarps], x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kUnitWarps; ++w) mm = fmaxf(mm, sml[w * D::ROWS + tr].x);
 #pragma unroll
       for (int w = 0; w < kUnitWarps; ++w) {
         const float2 ml = sml[w * D::ROWS + tr];
-        const float f = weight_of(ml.x, mm, st.lg);
+        f[w] = weight_of(ml.x, mm, st.lg);
+        l += f[w] * ml.y;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int w = 0; w < kUnitWarps; ++w) {
         const float4 v = *reinterpret_cast<const float4*>(so + (w * D::ROWS + tr) * DV + e);
-        l += f * ml.y;
-        x[0] += f * v.x, x[1] += f * v.y, x[2] += f * v.z, x[3] += f * v.w;
+        const float g = f[w] * inv * sunit[w];
+        x[0] += g * v.x, x[1] += g * v.y, x[2] += g * v.z, x[3] += g * v.w;
       }
       if (it.part >= 0) {
         if (e == 0) a.plan.ml[part + tr] = make_float2(mm, l);
         *reinterpret_cast<float4*>(a.plan.o + (part + tr) * DV + e) = make_float4(x[0], x[1], x[2], x[3]);
       } else {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] *= inv;
         out_store4(static_cast<T*>(a.call.out) + row.x * a.call.out_stride[0] +
                        (int64_t)(head * a.shape.share + row.w) * a.call.out_stride[1] + e,
                    ovec, x);

@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) attend8_tile_ke
     asm volatile("bar.sync 5, 256;" ::: "memory");
     l += maxima[(1 - half) * kRows + trow];
     const size_t part = ((size_t)max(it.part, 0) * H + head) * kRows + trow;
-    const float f = it.part >= 0 ? unit : l == 0.f ? 0.f : unit / l;
+    const float f = l == 0.f ? 0.f : unit / l;
     const bool ovec = a.call.out_stride[0] % 4 == 0 && a.call.out_stride[1] % 4 == 0 &&
                       (reinterpret_cast<uintptr_t>(a.call.out) & 7) == 0;
     bf16* out = static_cast<bf16*>(a.call.out) + row.x * a.call.out_stride[0] +

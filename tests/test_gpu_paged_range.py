@@ -159,3 +159,23 @@ def test_values_at_both_ends_of_the_range(rows, dtype):
     w = np.where(big, math.exp(7.0), 1.0)
     want = np.full((seqs * rows, heads, 64), 2.0**110 * w[big].sum() / w.sum())
     _check(got, want, want, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("shape", list(SHAPES))
+def test_values_of_the_largest_size(shape, dtype):
+    """Values at the upper end of fp32 average to values of that size: no sum
+    over keys, warps or parts runs over."""
+    rng, pool, plan, seqs, nrow, vis = _step(shape, dtype, 11)
+    pool.begin_pages(list(range(pool.num_pages)))
+    slots = np.concatenate(seqs)
+    k = torch.zeros((len(slots), 1, 64), device=DEV)
+    v = torch.tensor(rng.choice([3e38, 2e38, 1.5e38], (len(slots), 1, 64)), dtype=torch.float32, device=DEV)
+    v[..., 32:] *= -1
+    paged.kv_append(pool, 0, paged.AppendPlan(pool, slots), k, v)
+    q = torch.zeros((len(vis), 2, 64), dtype=dtype, device=DEV)
+    got = paged.paged_attention(pool, 0, plan, q)
+    paged.check_status(pool)
+    means = np.stack([_f64(paged.kv_read(pool, 0, s, torch.float32)[1][:, 0]).mean(0) for s in seqs])
+    want = np.repeat(means, nrow, axis=0)[:, None].repeat(2, 1)
+    _check(got, want, np.abs(want), dtype)
