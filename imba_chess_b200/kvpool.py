@@ -28,7 +28,9 @@ pairs, ``[H][8][d_v][2]``) and ``scales`` the scales' exponents, one byte per
 block (0: an empty block).  A block's scale grows with its tokens and never
 shrinks, so pages start afresh when they are handed out: ``alloc`` notes them
 and ``begin_pages`` clears their scales on the stream of the next call that
-writes to the pool.  ``imba_chess_b200.paged`` has the operators on a pool.
+writes to the pool.  Those pages may be another stream's, before and after, so
+that clearing waits for what the pool's other streams have enqueued, and their
+next calls wait for it.  ``imba_chess_b200.paged`` has the operators on a pool.
 """
 
 from __future__ import annotations
@@ -73,6 +75,9 @@ class KVPool:
             self.data = torch.zeros((self.num_pages, self.page_elems), dtype=dtype, device=device)
         self._free = np.arange(self.num_pages - 1, -1, -1, dtype=np.int64).tolist()
         self._fresh: list[int] = []  # pages in 8 bits handed out since begin_pages()
+        self._streams: dict[int, torch.cuda.Stream] = {}  # that calls on a pool in 8 bits ran on, by handle
+        self._ordered: set[int] = set()  # of them, those behind the last begin_pages()
+        self._begun_on: torch.cuda.Stream | None = None  # where that one ran
         self.desc = _native.PoolDesc(self.data.data_ptr(), self.num_pages)
 
     @property
@@ -102,7 +107,9 @@ class KVPool:
         """Empty the blocks of ``pages`` (default: the pages handed out since
         the last call) of a pool in 8 bits, on the current stream.  The
         operators and the model's steps call this; a caller that recycles
-        pages without ``alloc``, or captures a CUDA graph after one, does."""
+        pages without ``alloc``, or captures a CUDA graph after one, does.
+        Behind all that the pool's other streams have enqueued (a graph's
+        replays are not known here: order them yourself)."""
         if self.scales is None:
             return
         if pages is None:
@@ -114,7 +121,28 @@ class KVPool:
         ids = torch.as_tensor(pages, dtype=torch.int64)
         if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= self.num_pages):
             raise ValueError("begin_pages: page id outside the pool")
+        if self.data.is_cuda:
+            stream = torch.cuda.current_stream(self.data.device)
+            self._streams[stream.cuda_stream] = stream
+            for other in self._streams.values():
+                if other.cuda_stream != stream.cuda_stream:
+                    stream.wait_stream(other)
+            self._ordered = {stream.cuda_stream}
+            self._begun_on = stream
         self.scales.index_fill_(0, ids.to(self.device), 0)
+
+    def join_stream(self) -> None:
+        """The current stream is one that works on this pool in 8 bits: its
+        next work comes after the last ``begin_pages``, and the next
+        ``begin_pages`` after its work."""
+        stream = torch.cuda.current_stream(self.data.device)
+        with torch.cuda.device(self.data.device):
+            if torch.cuda.is_current_stream_capturing():
+                return  # (a capture cannot wait for work outside of it)
+        if self._begun_on is not None:
+            stream.wait_stream(self._begun_on)
+        self._streams[stream.cuda_stream] = stream
+        self._ordered.add(stream.cuda_stream)
 
     def release_pages(self, pages: list[int]) -> None:
         self._free.extend(reversed(pages))

@@ -189,9 +189,9 @@ class B200HSTUChessModel:
         desc.status = ptr(status if status is not None else self._status)
         ws = self.workspace(rows)
         s = stream if stream is not None else torch.cuda.current_stream(self.device)
-        if pool._fresh:
+        if pool._fresh or (pool.scales is not None and s.cuda_stream not in pool._ordered):
             with torch.cuda.stream(s):
-                pool.begin_pages()
+                pool.begin_pages() if pool._fresh else pool.join_stream()
         with torch.cuda.device(self.device):
             code = self._lib.imba_step(self._handle, ctypes.byref(desc), ctypes.byref(pool.desc), ws.data_ptr(),
                                        ws.numel(), s.cuda_stream)
@@ -231,6 +231,8 @@ class B200HSTUChessModel:
         k = torch.empty((n, d.num_heads, d.attention_dim), dtype=self.dtype, device=self.device)
         v = torch.empty((n, d.num_heads, d.linear_dim), dtype=self.dtype, device=self.device)
         s = torch.cuda.current_stream(self.device)
+        if pool.scales is not None and s.cuda_stream not in pool._ordered:
+            pool.join_stream()
         with torch.cuda.device(self.device):
             code = self._lib.imba_kv_gather(self._handle, ctypes.byref(pool.desc), layer, n, slots.data_ptr(),
                                             k.data_ptr(), v.data_ptr(), self._status.data_ptr(), s.cuda_stream)

@@ -23,7 +23,8 @@ A plan keeps the tensors it was made from and its scratch: calls on one plan
 must not overlap (two streams, two captured graphs), and the plan's tensors
 hold the step's rows as they were when it was made.  A call on another stream
 than the plan's waits for nothing by itself, as with any tensor, and marks the
-plan's memory as used there; a captured graph needs its plans kept alive.
+plan's memory as used there; a captured graph needs its plans kept alive.  A
+pool in 8 bits orders its streams where it empties pages (``kvpool``).
 """
 
 from __future__ import annotations
@@ -84,6 +85,8 @@ def _call(pool: KVPool, what: str, *args, plan=None) -> None:
     index = pool.data.get_device()
     fn = _FNS.get(what) or _FNS.setdefault(what, getattr(_native.load(), what))
     stream = _raw_stream(index)
+    if pool.scales is not None and stream not in pool._ordered:
+        pool.join_stream()
     if plan is not None and stream != plan._stream:
         _used_on(plan, index)
     if torch.cuda.current_device() == index:

@@ -1,0 +1,93 @@
+"""GPU: a pool in 8 bits used on several streams, and what its host calls wait for."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from imba_chess_b200 import paged
+from imba_chess_b200.kvpool import KVSequence
+from tests.test_gpu_paged import DEV, _pool
+
+pytestmark = pytest.mark.gpu
+
+LONG = 400_000_000  # cycles of the device: some 0.2 s
+
+
+def _step(pool, rows, seed):
+    """A sequence of ``rows`` new tokens: (sequence, its append plan, keys and values, queries, its attention plan)."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    rand = lambda: torch.randn((rows, 2, 64), dtype=torch.bfloat16, device=DEV, generator=gen)  # noqa: E731
+    seq = KVSequence(pool)
+    slots = seq.reserve(rows)
+    plan = paged.AppendPlan(pool, slots)
+    sees = paged.AttentionPlan(pool, row_off=[0, rows], row_vis=list(range(1, rows + 1)), page_off=[0, len(seq.pages)],
+                               pages=seq.pages, num_q_heads=2)
+    return seq, plan, (rand(), rand()), rand(), sees
+
+
+def test_pages_are_emptied_behind_their_last_readers():
+    """A page that one stream still reads comes back to the pool and is handed
+    out again: a step of another stream does not empty it under the reader."""
+    pool = _pool(pages=4)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    b.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(b):
+        seq, plan, kv, q, sees = _step(pool, 10, 1)
+        paged.kv_append(pool, 0, plan, *kv)
+        want = paged.paged_attention(pool, 0, sees, q)
+    torch.cuda.synchronize()
+    assert want.any()
+    with torch.cuda.stream(b):
+        torch.cuda._sleep(LONG)
+        got = paged.paged_attention(pool, 0, sees, q)
+    page = seq.pages[0]
+    seq.release()
+    again = KVSequence(pool)
+    again.reserve(3)
+    assert again.pages == [page]  # for stream b's next step
+    with torch.cuda.stream(a):
+        _, plan_a, kv_a, _, _ = _step(pool, 5, 2)
+        paged.kv_append(pool, 0, plan_a, *kv_a)
+    torch.cuda.synchronize()
+    paged.check_status(pool)
+    assert torch.equal(got, want)
+
+
+def test_pages_are_emptied_before_other_streams_write():
+    """One stream's step empties the pages of another's, which waits for it."""
+    pool, alone = _pool(pages=4), _pool(pages=4)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for s in (a, b):
+        s.wait_stream(torch.cuda.current_stream())
+    _, plan_a, kv_a, _, _ = _step(pool, 5, 1)
+    seq, plan_b, kv_b, _, _ = _step(pool, 20, 2)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(LONG)
+        paged.kv_append(pool, 0, plan_a, *kv_a)
+    with torch.cuda.stream(b):
+        paged.kv_append(pool, 0, plan_b, *kv_b)
+    torch.cuda.synchronize()
+    paged.check_status(pool)
+    slots = seq.slots(0, 20)
+    paged.kv_append(alone, 0, paged.AppendPlan(alone, slots), *kv_b)
+    for got, want in zip(paged.kv_read(pool, 0, slots), paged.kv_read(alone, 0, slots)):
+        assert torch.equal(got, want) and got.any()
+
+
+def test_graphs_on_their_own_stream():
+    """A capture waits for no other stream; its replays are the caller's to order."""
+    pool = _pool(pages=4)
+    seq, plan, kv, q, sees = _step(pool, 10, 1)
+    paged.kv_append(pool, 0, plan, *kv)
+    want = paged.paged_attention(pool, 0, sees, q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        paged.kv_append(pool, 0, plan, *kv)
+        got = paged.paged_attention(pool, 0, sees, q)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    paged.check_status(pool)
+    assert torch.equal(got, want)
