@@ -49,6 +49,20 @@ class KVPoolExhausted(RuntimeError):
     """The pool has fewer free pages than a request needs."""
 
 
+def to_device(host: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """A host tensor's copy on ``device``, enqueued on its current stream: the
+    host goes on at once, through pinned memory that is not handed out again
+    before the copy is done."""
+    if device.type != "cuda" or host.numel() == 0:
+        return host.to(device)
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("host data cannot be copied in a capture (its replays would copy it again): "
+                               "put it on the device before")
+        pinned = torch.empty(host.shape, dtype=host.dtype, pin_memory=True)
+        return pinned.copy_(host).to(device, non_blocking=True)
+
+
 class KVPool:
     def __init__(self, *, num_layers: int, num_heads: int, attention_dim: int, linear_dim: int,
                  num_pages: int, dtype: torch.dtype, device: torch.device) -> None:
@@ -110,15 +124,15 @@ class KVPool:
         pages without ``alloc``, or captures a CUDA graph after one, does.
         Behind all that the pool's other streams have enqueued (a graph's
         replays are not known here: order them yourself)."""
-        if self.scales is None:
+        if self.scales is None or (pages is None and not self._fresh):
             return
+        if self.data.is_cuda:
+            with torch.cuda.device(self.data.device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("pages are not emptied in a capture: call pool.begin_pages() before the capture")
         if pages is None:
-            if not self._fresh:
-                return
-            if self.data.is_cuda and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("pages were handed out since the last step: call pool.begin_pages() before the capture")
             pages, self._fresh = self._fresh, []
-        ids = torch.as_tensor(pages, dtype=torch.int64)
+        ids = torch.as_tensor(pages, dtype=torch.int64).cpu()
         if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= self.num_pages):
             raise ValueError("begin_pages: page id outside the pool")
         if self.data.is_cuda:
@@ -129,7 +143,7 @@ class KVPool:
                     stream.wait_stream(other)
             self._ordered = {stream.cuda_stream}
             self._begun_on = stream
-        self.scales.index_fill_(0, ids.to(self.device), 0)
+        self.scales.index_fill_(0, to_device(ids, self.data.device), 0)
 
     def join_stream(self) -> None:
         """The current stream is one that works on this pool in 8 bits: its

@@ -15,7 +15,8 @@ every layer::
 They stand beside ``B200HSTUChessModel.kv_scatter`` / ``kv_gather`` (rows of a
 model's own pool, as they are); a model with ``kv_dtype=torch.float8_e4m3fn``
 runs its steps on them.  Everything is enqueued on the current stream of the
-pool's device and nothing waits for the device: what only the device can see
+pool's device and nothing but ``check_status`` waits for the device (host lists
+and arrays are copied through pinned memory): what only the device can see
 (a slot or a page outside the pool, a row that is not finite) is skipped,
 written to ``pool``'s status word and raised by ``check_status(pool)``.
 
@@ -37,7 +38,7 @@ from fractions import Fraction
 import torch
 
 from . import _native
-from .kvpool import PAGE, KVPool
+from .kvpool import PAGE, KVPool, to_device
 
 _PI = Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
 _DTYPES = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16}
@@ -119,7 +120,9 @@ def _ints(x, pool: KVPool, what: str, shape: tuple[int, ...] | None = None) -> t
         raise ValueError(f"{what} is on {t.device}, the pool on {pool.data.device}")
     if shape is not None and tuple(t.shape) != shape:
         raise ValueError(f"{what} must have shape {shape}, got {tuple(t.shape)}")
-    return t.to(device=pool.data.device, dtype=torch.int32).contiguous()
+    if not t.is_cuda:
+        return to_device(t.to(torch.int32).contiguous(), pool.data.device)
+    return t.to(torch.int32).contiguous()
 
 
 def _rows(t: torch.Tensor, pool: KVPool, what: str, shape: tuple[int, ...], dtype) -> None:

@@ -91,3 +91,57 @@ def test_graphs_on_their_own_stream():
     torch.cuda.synchronize()
     paged.check_status(pool)
     assert torch.equal(got, want)
+
+
+def test_nothing_waits_for_the_device():
+    """Pages handed out, plans from host lists, append, attention and reads
+    are enqueued while the device is busy with something else."""
+    pool = _pool(pages=8)
+    _, plan, kv, q, sees = _step(pool, 10, 1)  # the first use: libraries and memory
+    paged.kv_append(pool, 0, plan, *kv)
+    paged.paged_attention(pool, 0, sees, q)
+    slots = KVSequence(pool).reserve(10)
+    paged.kv_read(pool, 0, slots)
+    _, plan, kv, q, sees = _step(pool, 40, 2)
+    paged.kv_append(pool, 0, plan, *kv)
+    torch.cuda.synchronize()
+    busy = torch.cuda.Event()
+    torch.cuda._sleep(10 * LONG)
+    busy.record()
+    seq, plan, kv, q, sees = _step(pool, 20, 3)
+    paged.kv_append(pool, 0, plan, *kv)
+    got = paged.paged_attention(pool, 0, sees, q)
+    read = paged.kv_read(pool, 0, seq.slots(0, 20))
+    assert not busy.query()
+    torch.cuda.synchronize()
+    paged.check_status(pool)
+    alone = _pool(pages=8)
+    plan = paged.AppendPlan(alone, seq.slots(0, 20))
+    paged.kv_append(alone, 0, plan, *kv)
+    for mine, want in zip(read, paged.kv_read(alone, 0, seq.slots(0, 20))):
+        assert torch.equal(mine, want)
+    sees = paged.AttentionPlan(alone, row_off=[0, 20], row_vis=list(range(1, 21)), page_off=[0, 2], pages=seq.pages, num_q_heads=2)
+    assert torch.equal(got, paged.paged_attention(alone, 0, sees, q))
+
+
+def test_host_data_is_copied_when_it_is_given():
+    """What a caller does with its arrays afterwards, pinned ones too, changes
+    nothing; and a capture takes no host data."""
+    pool = _pool(pages=8)
+    slots = torch.arange(20, dtype=torch.int32).pin_memory()
+    torch.cuda._sleep(LONG)
+    plan = paged.AppendPlan(pool, slots)
+    slots.fill_(3)
+    torch.cuda.synchronize()
+    assert plan.slots.tolist() == list(range(20))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="capture"):
+            paged.AppendPlan(pool, [0, 1])
+        with pytest.raises(RuntimeError, match="capture"):
+            pool.begin_pages([0])
+        keep = paged.AppendPlan(pool, plan.slots)
+    graph.replay()
+    torch.cuda.synchronize()
+    paged.check_status(pool)
+    del keep
