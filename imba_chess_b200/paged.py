@@ -110,7 +110,9 @@ def _used_on(plan, index: int) -> None:
 
 
 def _ints(x, pool: KVPool, what: str, shape: tuple[int, ...] | None = None) -> torch.Tensor:
-    """A contiguous int32 tensor on the pool's device."""
+    """A contiguous int32 tensor on the pool's device.  Wider integers that are
+    on the device already are clamped, not wrapped: what was outside int32 is
+    then outside every pool and is reported there."""
     t = torch.as_tensor(x)
     if t.numel() and (t.is_floating_point() or t.is_complex() or t.dtype == torch.bool):
         raise ValueError(f"{what} must be integers")
@@ -122,6 +124,10 @@ def _ints(x, pool: KVPool, what: str, shape: tuple[int, ...] | None = None) -> t
         raise ValueError(f"{what} must have shape {shape}, got {tuple(t.shape)}")
     if not t.is_cuda:
         return to_device(t.to(torch.int32).contiguous(), pool.data.device)
+    if t.dtype == torch.int64:
+        t = t.clamp(-(2**31), 2**31 - 1)
+    elif t.dtype in (torch.uint32, torch.uint64):
+        raise ValueError(f"{what} on the device must be int32 or int64, got {t.dtype}")
     return t.to(torch.int32).contiguous()
 
 

@@ -1,0 +1,45 @@
+"""GPU: calls of the cache operators that the documentation allows, or refuses."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from imba_chess_b200 import _native, paged
+from tests.test_gpu_paged import DEV, _check_stored, _f64, _fill, _pool, _rand
+
+pytestmark = pytest.mark.gpu
+
+
+def _reported(pool):
+    with pytest.raises(_native.ImbaError) as e:
+        paged.check_status(pool)
+    assert e.value.code == _native.IMBA_ERR_RANGE
+    paged.check_status(pool)
+
+
+@pytest.mark.parametrize("far", [2**32 + 5, 2**31, -(2**32) + 5, -(2**40), 2**63 - 1])
+def test_wide_integers_on_the_device(far):
+    """int64 tensors on the device are taken by value: what is outside int32
+    is outside the pool, and is skipped and reported."""
+    rng = np.random.default_rng(1)
+    pool = _pool(pages=4)
+    k, v = (_rand(rng, (3, 2, 64), torch.float32) for _ in range(2))
+    wide = lambda *x: torch.tensor(x, dtype=torch.int64, device=DEV)  # noqa: E731
+    paged.kv_append(pool, 0, paged.AppendPlan(pool, wide(5, 20, -1)), k, v)
+    paged.check_status(pool)
+    paged.kv_append(pool, 0, paged.AppendPlan(pool, wide(4, far, 21)), k, v)
+    _reported(pool)
+    kept = {5: (_f64(k[0]), _f64(v[0])), 20: (_f64(k[1]), _f64(v[1])), 4: (_f64(k[0]), _f64(v[0])), 21: (_f64(k[2]), _f64(v[2]))}
+    _check_stored(pool, 0, kept)
+    paged.kv_read(pool, 0, wide(5, far))
+    _reported(pool)
+    rows = dict(row_off=wide(0, 1), row_vis=wide(6), page_off=wide(0, 1), pages=wide(0), num_q_heads=2)
+    q = _rand(rng, (1, 2, 64))
+    want = paged.paged_attention(pool, 0, paged.AttentionPlan(pool, **rows), q)
+    paged.check_status(pool)
+    assert want.any()
+    for name, bad in (("pages", wide(far)), ("row_vis", wide(far)), ("row_off", wide(0, far)), ("page_off", wide(0, far))):
+        paged.paged_attention(pool, 0, paged.AttentionPlan(pool, **{**rows, name: bad}), q)
+        _reported(pool)
