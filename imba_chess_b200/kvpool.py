@@ -92,6 +92,8 @@ class KVPool:
         self._streams: dict[int, torch.cuda.Stream] = {}  # that calls on a pool in 8 bits ran on, by handle
         self._ordered: set[int] = set()  # of them, those behind the last begin_pages()
         self._begun_on: torch.cuda.Stream | None = None  # where that one ran
+        # what the operators on the pool report to (made here: in a capture, each replay would clear it)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self.desc = _native.PoolDesc(self.data.data_ptr(), self.num_pages)
 
     @property

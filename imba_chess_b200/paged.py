@@ -61,8 +61,7 @@ def _cache(pool: KVPool):
             raise ValueError("the cache operators take head dimensions up to 128")
         desc = _native.CacheDesc(pool.num_layers, pool.num_heads, pool.attention_dim, pool.linear_dim,
                                  _POOL_DTYPES[pool.dtype])
-        status = torch.zeros(1, dtype=torch.int32, device=pool.device)
-        got = pool._cache = (ctypes.byref(desc), ctypes.byref(pool.desc), status, desc)
+        got = pool._cache = (ctypes.byref(desc), ctypes.byref(pool.desc), pool.status, desc)
     return got
 
 

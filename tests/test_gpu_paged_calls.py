@@ -43,3 +43,23 @@ def test_wide_integers_on_the_device(far):
     for name, bad in (("pages", wide(far)), ("row_vis", wide(far)), ("row_off", wide(0, far)), ("page_off", wide(0, far))):
         paged.paged_attention(pool, 0, paged.AttentionPlan(pool, **{**rows, name: bad}), q)
         _reported(pool)
+
+
+def test_errors_of_a_graph_that_is_the_first_use():
+    """A pool whose first operators are captured: what a replay reports stays
+    until it is read, through further replays."""
+    rng = np.random.default_rng(2)
+    warm = _pool(pages=4)
+    k, v = (_rand(rng, (2, 2, 64)) for _ in range(2))
+    paged.kv_append(warm, 0, paged.AppendPlan(warm, [0, 1]), k, v)
+    pool = _pool(pages=4)
+    slots = torch.tensor([0, 9999], dtype=torch.int32, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan = paged.AppendPlan(pool, slots)
+        paged.kv_append(pool, 0, plan, k, v)
+    graph.replay()
+    slots.copy_(torch.tensor([0, 1], dtype=torch.int32))
+    graph.replay()
+    _reported(pool)
+    _check_stored(pool, 0, {i: (_f64(k[i]), _f64(v[i])) for i in (0, 1)})
