@@ -57,7 +57,8 @@ size_t workspace_layout(const imba_model* m, int32_t rows, void* base, Workspace
   w.kv_slots = static_cast<int*>(take(m->cache8 ? R * sizeof(int) : 0));
   w.append_bytes = m->cache8 ? imba_append_plan_bytes((int32_t)R) : 0;
   w.append_plan = take(w.append_bytes);
-  w.attend_plan = take(m->cache8 ? attend_step_bytes(m->cache(), (int32_t)R) : 0);
+  w.attend_bytes = m->cache8 ? attend_step_bytes(m->cache(), (int32_t)R) : 0;
+  w.attend_plan = take(w.attend_bytes);
   w.bytes = off;
   if (ws) *ws = w;
   return off;
@@ -195,6 +196,7 @@ cudaError_t begin_cache8(const imba_model* m, const imba_step_desc& st, const im
   t.rows.status = st.status;
   t.shape = attend_shape(c->cache, t.rows, attend_step_most(st.num_rows));
   t.plan = attend_plan_view(c->cache, t.rows, t.shape, w.attend_plan);
+  if (t.plan.bytes > w.attend_bytes) return cudaErrorInvalidValue;  // (attend_step_bytes covers every step)
   t.call = {};
   t.call.dtype = md.dtype;
   t.call.q = w.q;

@@ -218,6 +218,9 @@ namespace {
 // up to 600 tokens turn at about the same numbers of rows.)
 constexpr int64_t kTileFrom = 80;
 
+// Head sizes of that kernel.
+bool tile_dims(const imba_cache_desc& c) { return c.attention_dim == c.linear_dim && c.attention_dim % 64 == 0; }
+
 // The shape with tiles of 8 rt rows and `warps` warps a unit.
 AttendShape shape_of(const imba_cache_desc& c, const imba_attend_desc& r, int rt, int warps, int64_t most) {
   AttendShape sh;
@@ -253,8 +256,7 @@ AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r, in
   // hold it (the games' step, one row a segment: 44 us with one group, 48 with
   // two; waves of siblings: 54 with one, 43 with two).
   const int64_t per_seg = r.num_segs ? (flat + r.num_segs - 1) / r.num_segs : 0;
-  if (r.num_extra == 0 && c.attention_dim == c.linear_dim && c.attention_dim % 64 == 0 && per_seg >= kTileFrom)
-    return shape_of(c, r, kTileGroups, kUnitWarps, most);
+  if (r.num_extra == 0 && tile_dims(c) && per_seg >= kTileFrom) return shape_of(c, r, kTileGroups, kUnitWarps, most);
   // Three groups only where they save a tile of two (20 rows a segment, bf16,
   // 131,000 tokens, 8 heads of 128: 79 us against 157; 512 segments of up to
   // 600 tokens, 4 heads of 64: 79 against 80; with 33 to 60 rows a segment,
@@ -271,13 +273,24 @@ AttendShape attend_shape(const imba_cache_desc& c, const imba_attend_desc& r, in
 
 size_t attend_step_bytes(const imba_cache_desc& c, int32_t rows) {
   imba_attend_desc r = {};
-  r.num_rows = r.num_segs = r.num_groups = rows;  // every chunk holds a row
+  r.num_rows = r.num_groups = rows;
   r.num_group_pages = kMostPages;
   r.num_q_heads = c.num_heads;
   size_t most = 0;
-  for (int rt : {1, 2, 3, kTileGroups})
-    for (int warps : {1, kUnitWarps})
+  // What attend_shape gives such a step: a tile size comes with segments of
+  // more rows than `past` on average, so there are (rows - 1) / past at most,
+  // and every part of a plan grows with their number.
+  auto add = [&](int rt, int warps, int past) {
+    r.num_segs = past ? (rows - 1) / past : rows;
+    if (r.num_segs > 0)
       most = std::max(most, attend_plan_view(c, r, shape_of(c, r, rt, warps, attend_step_most(rows)), nullptr).bytes);
+  };
+  for (int warps : {1, kUnitWarps}) {
+    add(1, warps, 0);
+    add(2, warps, 8);
+    add(3, warps, 16);
+  }
+  if (tile_dims(c)) add(kTileGroups, kUnitWarps, kTileFrom - 1);
   return most;
 }
 

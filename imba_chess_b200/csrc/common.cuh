@@ -161,6 +161,7 @@ struct Workspace {
   void* append_plan;
   size_t append_bytes;
   void* attend_plan;
+  size_t attend_bytes;
   size_t bytes;
 };
 
