@@ -105,7 +105,7 @@ size_t imba_cache_pool_bytes(const imba_cache_desc* cache, int64_t num_pages) {
 }
 
 size_t imba_append_plan_bytes(int32_t num_rows) {
-  if (num_rows < 0 || num_rows > (1 << 28)) return 0;
+  if (num_rows < 0 || num_rows > imba::kMostRows) return 0;
   const int64_t cap = imba::plan_cap(num_rows);
   return (size_t)(imba::kPlanHead + cap * (1 + IMBA_PAGE_TOKENS) + num_rows) * sizeof(int32_t);
 }
@@ -114,7 +114,7 @@ imba_status_t imba_append_plan(const imba_pool_desc* pool, int32_t num_rows, con
                                size_t plan_bytes, int32_t* status, void* stream) {
   const imba_status_t v = imba::validate_pool(pool);
   if (v != IMBA_OK) return v;
-  if (num_rows < 0 || num_rows > (1 << 28)) return IMBA_ERR_ARG;
+  if (num_rows < 0 || num_rows > imba::kMostRows) return IMBA_ERR_ARG;
   if (!plan || (num_rows > 0 && !slots) || (reinterpret_cast<uintptr_t>(plan) & 255)) return IMBA_ERR_ARG;
   if (plan_bytes < imba_append_plan_bytes(num_rows)) return IMBA_ERR_OOM;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -128,7 +128,7 @@ imba_status_t imba_kv_append(const imba_cache_desc* cache, const imba_pool_desc*
   imba_status_t v = imba::validate_cache(cache);
   if (v == IMBA_OK) v = imba::validate_pool(pool);
   if (v != IMBA_OK) return v;
-  if (!append || append->num_rows < 0) return IMBA_ERR_ARG;
+  if (!append || append->num_rows < 0 || append->num_rows > imba::kMostRows) return IMBA_ERR_ARG;
   if (append->layer < 0 || append->layer >= cache->num_layers) return IMBA_ERR_RANGE;
   if (append->src_dtype != IMBA_DTYPE_F32 && append->src_dtype != IMBA_DTYPE_BF16) return IMBA_ERR_ARG;
   if (append->num_rows == 0) return IMBA_OK;

@@ -17,6 +17,7 @@ constexpr float kLargest = 3.19014718988379809496e38f;  // 1.875 2^127
 // table's keys [cap], the rows of each key's page [cap][16], and the list of
 // occupied table positions [num_rows].
 constexpr int kPlanHead = 64;
+constexpr int kMostRows = 1 << 28;  // of a step: plan_cap is an int32
 inline int plan_cap(int32_t n) {
   int cap = 64;
   while (cap < 2 * (int64_t)n) cap *= 2;

@@ -328,7 +328,8 @@ IMBA_API size_t imba_cache_pool_bytes(const imba_cache_desc* cache, int64_t num_
  * layer.  Row r goes to slot slots[r]; -1 is a padding
  * row, which is passed over; other slots outside the pool are skipped and
  * reported (IMBA_ERR_RANGE).  Of rows with the same slot the last one is
- * stored.  `plan` is device memory, 256-byte aligned. */
+ * stored.  A step has at most 2^28 rows (IMBA_ERR_ARG; 0 bytes).  `plan` is
+ * device memory, 256-byte aligned. */
 IMBA_API size_t imba_append_plan_bytes(int32_t num_rows);
 IMBA_API imba_status_t imba_append_plan(const imba_pool_desc* pool, int32_t num_rows, const int32_t* slots,
                                         void* plan, size_t plan_bytes, int32_t* status, void* stream);
