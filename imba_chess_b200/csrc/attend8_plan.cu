@@ -18,27 +18,28 @@ constexpr int kPlanThreads = 1024;
 inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Exclusive sum over the CTA's threads; the total in *total.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
+template <typename I>
+__device__ __forceinline__ I block_scan(I v, I* warp_sums, I* total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  int x = v;
+  I x = v;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    const I y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    int w = lane < kPlanThreads / 32 ? warp_sums[lane] : 0;
+    I w = lane < kPlanThreads / 32 ? warp_sums[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
-      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      const I y = __shfl_up_sync(0xffffffffu, w, o);
       if (lane >= o) w += y;
     }
     warp_sums[lane] = w;
   }
   __syncthreads();
-  const int before = (warp ? warp_sums[warp - 1] : 0) + x - v;
+  const I before = (warp ? warp_sums[warp - 1] : 0) + x - v;
   *total = warp_sums[kPlanThreads / 32 - 1];
   __syncthreads();
   return before;
@@ -102,28 +103,29 @@ __device__ __forceinline__ int most_parts(int pages, int rt) {
 __global__ void __launch_bounds__(kPlanThreads) attend_items_kernel(imba_attend_desc r, AttendShape sh, AttendPlan p,
                                                                     int H) {
   __shared__ int warp_sums[32];
+  __shared__ long long tile_sums[32];
   __shared__ unsigned long long all_pages;
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x;
   if (tid == 0) all_pages = 0;
-  // Tiles of each segment.
-  int ntiles = 0;
+  // Tiles of each segment, counted in 64 bits: segments that overlap can ask
+  // for more rows than there are, each of them for all.
+  long long asked = 0;
   for (int s0 = 0; s0 < r.num_segs; s0 += kPlanThreads) {
     const int s = s0 + tid;
-    int off = 0, n = 0, t = 0, sum;
+    int off = 0, n = 0;
+    long long t = 0, sum;
     if (s < r.num_segs) {
       segment(r, s, &off, &n);
-      t = (int)(((int64_t)n * sh.share + sh.tile_rows - 1) / sh.tile_rows);
+      t = ((int64_t)n * sh.share + sh.tile_rows - 1) / sh.tile_rows;
     }
-    const int before = block_scan(t, warp_sums, &sum);
-    if (s < r.num_segs) p.tile_off[s] = min(ntiles + before, sh.max_tiles);
-    ntiles += sum;
+    const long long before = block_scan(t, tile_sums, &sum);
+    if (s < r.num_segs) p.tile_off[s] = (int)min(asked + before, (long long)sh.max_tiles);
+    asked += sum;
   }
-  if (ntiles > sh.max_tiles) {  // segments that overlap can ask for more rows than there are
-    if (tid == 0) report(r.status, IMBA_ERR_RANGE);
-    ntiles = sh.max_tiles;
-  }
+  if (asked > sh.max_tiles && tid == 0) report(r.status, IMBA_ERR_RANGE);
+  const int ntiles = (int)min(asked, (long long)sh.max_tiles);
   if (tid == 0) p.tile_off[r.num_segs] = ntiles;
   __syncthreads();
   // Their rows and visible pages.

@@ -63,3 +63,24 @@ def test_errors_of_a_graph_that_is_the_first_use():
     graph.replay()
     _reported(pool)
     _check_stored(pool, 0, {i: (_f64(k[i]), _f64(v[i])) for i in (0, 1)})
+
+
+@pytest.mark.parametrize("seqs", [65536, 65538])
+def test_sequences_that_overlap(seqs):
+    """Offsets that go back and forth over all rows, which ask for 2^32 tiles
+    and more: reported, and every row is still some sequence's."""
+    rng = np.random.default_rng(3)
+    rows = 1 << 21
+    pool = _pool(heads=1, dqk=32, dv=32, pages=2)
+    _, pages, _ = _fill(pool, rng, [16])
+    q = torch.randn((rows, 1, 32), dtype=torch.bfloat16, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    vis = torch.arange(rows, dtype=torch.int32, device=DEV) % 17
+    plan = paged.AttentionPlan(pool, row_off=[0, rows], row_vis=vis, page_off=[0, 1], pages=pages[:1], num_q_heads=1)
+    want = paged.paged_attention(pool, 0, plan, q)
+    paged.check_status(pool)
+    off = np.where(np.arange(seqs + 1) % 2 == 0, 0, rows)
+    plan = paged.AttentionPlan(pool, row_off=off, row_vis=vis, page_off=np.arange(seqs + 1), pages=np.repeat(pages[:1], seqs),
+                               num_q_heads=1)
+    got = paged.paged_attention(pool, 0, plan, q, out=torch.zeros_like(q))
+    _reported(pool)
+    assert torch.equal(got, want)
