@@ -104,7 +104,8 @@ imba_status_t validate_step(const imba_model* m, const imba_step_desc* st, const
   if (st->num_rows < 0 || st->num_groups < 0 || st->num_chunks < 0 || st->num_legal < 0 || st->num_extra < 0 ||
       st->num_group_pages < 0)
     return IMBA_ERR_ARG;
-  if (m->cache8 && (st->num_group_pages > kMostPages || m->d.max_pos > kMostPos)) return IMBA_ERR_RANGE;
+  if (m->cache8 && (st->num_group_pages > kMostPages || st->num_extra > kMostExtra || m->d.max_pos > kMostPos))
+    return IMBA_ERR_RANGE;
   if (st->num_rows == 0) return IMBA_OK;
   if (st->num_chunks > st->num_rows) return IMBA_ERR_ARG;  // every chunk holds at least one row
   if (!pool->base || pool->num_pages <= 0) return IMBA_ERR_ARG;

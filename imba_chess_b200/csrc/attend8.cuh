@@ -27,6 +27,9 @@ constexpr int attend8_ctas(int dqk, int rt) {
 // position below -kMostPos puts every key into the last column, as it does.
 constexpr int kMostPages = 1 << 26;
 constexpr int kMostPos = 1 << 28;
+// Extra keys of a step: the rows of a warp (24 at most) can each ask for all,
+// and their sum is 32 bits.
+constexpr int kMostExtra = 1 << 26;
 
 struct AttendRow {  // one flattened row of a tile
   int row;          // -1: none

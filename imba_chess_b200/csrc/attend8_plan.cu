@@ -335,7 +335,7 @@ imba_status_t validate_rows(const imba_cache_desc* c, const imba_attend_desc* r)
   if (!r || r->num_rows < 0 || r->num_segs < 0 || r->num_groups < 0 || r->num_group_pages < 0 || r->num_extra < 0)
     return IMBA_ERR_ARG;
   if (r->num_q_heads <= 0 || r->num_q_heads % c->num_heads) return IMBA_ERR_ARG;
-  if (r->num_group_pages > kMostPages) return IMBA_ERR_RANGE;
+  if (r->num_group_pages > kMostPages || r->num_extra > kMostExtra) return IMBA_ERR_RANGE;
   if ((int64_t)r->num_rows * (r->num_q_heads / c->num_heads) > (1 << 28) || r->num_segs > (1 << 28))
     return IMBA_ERR_UNSUPPORTED;
   if (!r->seg_group && r->num_segs > r->num_groups) return IMBA_ERR_ARG;

@@ -313,7 +313,7 @@ class AttentionPlan:
         d.status = status.data_ptr()
         need = int(_native.load().imba_attend_plan_bytes(cache, ctypes.byref(d)))
         if need == 0:
-            raise ValueError("too many rows or pages for one step")
+            raise ValueError("too many rows, pages or extra keys for one step")
         self._plan = torch.empty(need, dtype=torch.uint8, device=pool.data.device)
         self._args = ctypes.create_string_buffer(_ATTEND.size)
         self._refs = (ctypes.byref(d), ctypes.cast(self._args, ctypes.POINTER(_native.AttendArgs)),

@@ -387,7 +387,7 @@ typedef struct imba_attend_desc {
   int32_t num_segs;
   int32_t num_groups;
   int32_t num_group_pages;          /* at most 2^26                                  */
-  int32_t num_extra;
+  int32_t num_extra;                /* at most 2^26                                  */
   int32_t num_q_heads;              /* a multiple of the cache's heads               */
   const int32_t* seg_group;         /* [S], or NULL: segment s is of group s         */
   const int32_t* seg_row_off;       /* [S], or with seg_nrows NULL [S + 1] offsets   */
