@@ -136,6 +136,16 @@ def _rows(t: torch.Tensor, pool: KVPool, what: str, shape: tuple[int, ...], dtyp
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
+def _apart(t: torch.Tensor, what: str) -> None:
+    """An output whose elements share no memory (an expanded tensor's do)."""
+    need = 1
+    for stride, size in sorted(zip(t.stride(), t.shape)):
+        if size > 1:
+            if stride < need:
+                raise ValueError(f"{what} has elements that share memory: shape {tuple(t.shape)}, strides {t.stride()}")
+            need += stride * (size - 1)
+
+
 class Rotary:
     """Rotary positions: pair ``p`` of a head turns by ``positions[axis[p]] *
     inv_freq[p]`` radians.  ``inv_freq`` has one value per pair, in the order
@@ -203,8 +213,10 @@ def kv_append(pool: KVPool, layer: int, plan: AppendPlan, k: torch.Tensor, v: to
     """Store a step's keys ``[n, H, d_qk]`` and values ``[n, H, d_v]`` (fp32
     or bf16, any strides) in one layer of the pool, the keys rotated to
     ``positions`` (int32 ``[n]``, or ``[n, axes]``) when ``rotary`` is given.
-    ``q`` ``[n, q_heads, d_qk]`` is rotated along and returned (in ``q_out``,
-    which may be ``q``; rows without a slot are left as they were)."""
+    ``q`` ``[n, q_heads, d_qk]`` is rotated along and returned, in ``q_out`` or
+    a new tensor.  ``q_out`` may be ``q``, and shares no memory with what else
+    the call reads.  Rows without a slot are left as they were: in a new tensor
+    they hold nothing defined."""
     cache, desc, _, _ = _cache(pool)
     if plan.pool is not pool:
         raise ValueError("the plan was made for another pool")
@@ -223,6 +235,9 @@ def kv_append(pool: KVPool, layer: int, plan: AppendPlan, k: torch.Tensor, v: to
             q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
         else:
             _rows(q_out, pool, "q_out", q.shape, dtype)
+            _apart(q_out, "q_out")
+            if q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride():
+                raise ValueError("q_out overlaps q in another order")
         if q.numel():
             q_heads, q_ptrs, q_strides = q.shape[1], (q.data_ptr(), q_out.data_ptr()), (*q.stride(), *q_out.stride())
     elif q_out is not None:
@@ -255,7 +270,7 @@ def kv_append(pool: KVPool, layer: int, plan: AppendPlan, k: torch.Tensor, v: to
 def kv_read(pool: KVPool, layer: int, slots, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The tokens in ``slots`` as dense ``[n, H, d_qk]`` and ``[n, H, d_v]``,
     in the pool's type; from a pool in 8 bits in bf16, which holds every stored
-    value, or fp32."""
+    value, or fp32.  Rows of slots outside the pool hold nothing defined."""
     cache, desc, status, _ = _cache(pool)
     dtype = dtype or (torch.bfloat16 if pool.dtype == torch.float8_e4m3fn else pool.dtype)
     if dtype not in _DTYPES or (pool.dtype != torch.float8_e4m3fn and dtype != pool.dtype):
@@ -330,7 +345,8 @@ def paged_attention(pool: KVPool, layer: int, plan: AttentionPlan, q: torch.Tens
     contiguous) to ``out`` ``[n, q_heads, d_v]`` of the same type.  ``scale``
     is 1 / sqrt(d_qk) by default; ``bias`` is fp32 ``[q_heads, 2 max_pos -
     1]``, its column the key's position less the row's, clamped, plus max_pos
-    - 1.  A row that sees nothing gets zeros."""
+    - 1.  A row that sees nothing gets zeros; a row of no sequence is left as
+    it was, and holds nothing defined in a new tensor.  ``out`` may be ``q``."""
     cache, desc, _, _ = _cache(pool)
     if plan.pool is not pool:
         raise ValueError("the plan was made for another pool")
@@ -342,6 +358,7 @@ def paged_attention(pool: KVPool, layer: int, plan: AttentionPlan, q: torch.Tens
         out = torch.empty((n, heads, pool.linear_dim), dtype=dtype, device=q.device)
     else:
         _rows(out, pool, "out", (n, heads, pool.linear_dim), dtype)
+        _apart(out, "out")
     if q.stride(2) != 1 or out.stride(2) != 1:
         raise ValueError("the last dimension of q and out must be contiguous")
     column, max_pos = 0, 0

@@ -84,3 +84,57 @@ def test_sequences_that_overlap(seqs):
     got = paged.paged_attention(pool, 0, plan, q, out=torch.zeros_like(q))
     _reported(pool)
     assert torch.equal(got, want)
+
+
+def test_outputs_that_share_memory():
+    """Expanded outputs and other orders of the input's memory are refused;
+    strided ones, and the queries themselves, are not."""
+    rng = np.random.default_rng(4)
+    pool = _pool()
+    k, v, q = (_rand(rng, (4, h, 64)) for h in (2, 2, 4))
+    plan = paged.AppendPlan(pool, [0, 1, 2, 3])
+    base = torch.zeros(4 * 4 * 64, dtype=torch.bfloat16, device=DEV)
+    bad = [base[:256].view(1, 4, 64).expand(4, 4, 64), base[:256].view(4, 1, 64).expand(4, 4, 64),
+           base.as_strided((4, 4, 64), (256, 32, 1)), base.as_strided((4, 4, 64), (64, 64, 1))]
+    for out in bad:
+        with pytest.raises(ValueError, match="share memory"):
+            paged.kv_append(pool, 0, plan, k, v, q=q, q_out=out)
+    turned = q[:, :, :].as_strided((4, 4, 64), (64, 256, 1))
+    with pytest.raises(ValueError, match="overlaps q"):
+        paged.kv_append(pool, 0, plan, k, v, q=q, q_out=turned)
+    once = q[:1].expand(4, 4, 64)
+    with pytest.raises(ValueError, match="share memory"):
+        paged.kv_append(pool, 0, plan, k, v, q=once, q_out=once)
+    assert torch.equal(paged.kv_append(pool, 0, plan, k, v, q=once), once)  # (an input may be expanded)
+    odd = torch.zeros((4, 64, 4), dtype=torch.bfloat16, device=DEV).transpose(1, 2)
+    assert torch.equal(paged.kv_append(pool, 0, plan, k, v, q=q, q_out=odd), q)
+    tight = torch.zeros(4 * 265, dtype=torch.bfloat16, device=DEV).as_strided((4, 4, 64), (265, 67, 1))
+    assert torch.equal(paged.kv_append(pool, 0, plan, k, v, q=q, q_out=tight), q)
+    one = base[:256].view(1, 4, 64)[:, :1].expand(1, 1, 64)
+    assert paged.kv_append(pool, 0, paged.AppendPlan(pool, [9]), k[:1], v[:1], q=q[:1, :1], q_out=one) is one
+    for rows in (4, 90):  # both kernels
+        n = rows
+        sees = paged.AttentionPlan(pool, row_off=[0, n], row_vis=np.arange(n) % 5, page_off=[0, 1], pages=[0], num_q_heads=4)
+        qq = _rand(rng, (n, 4, 64), torch.bfloat16, 0.3)
+        for out in (qq[:1].expand(n, 4, 64), qq[:, :1].expand(n, 4, 64)):
+            with pytest.raises(ValueError, match="share memory"):
+                paged.paged_attention(pool, 0, sees, qq, out=out)
+        want = paged.paged_attention(pool, 0, sees, qq)
+        assert torch.equal(paged.paged_attention(pool, 0, sees, qq[:1].expand(n, 4, 64))[0], want[0])
+        assert paged.paged_attention(pool, 0, sees, qq, out=qq) is qq and torch.equal(qq, want)
+    paged.check_status(pool)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_attention_in_place_of_split_lists(dtype):
+    """The queries as the output, where several CTAs read a row."""
+    rng = np.random.default_rng(5)
+    pool = _pool(heads=1, pages=300)
+    page_off, pages, _ = _fill(pool, rng, [4000, 600])
+    for rows in (3, 20, 100):
+        row_off = np.array([0, rows, rows + 2])
+        plan = paged.AttentionPlan(pool, row_off=row_off, row_vis=np.r_[np.full(rows, 4000), 600, 30], page_off=page_off,
+                                   pages=pages, num_q_heads=2)
+        q = _rand(rng, (rows + 2, 2, 64), dtype, 0.3)
+        want = paged.paged_attention(pool, 0, plan, q)
+        assert torch.equal(paged.paged_attention(pool, 0, plan, q, out=q), want)
