@@ -138,6 +138,8 @@ def _rows(t: torch.Tensor, pool: KVPool, what: str, shape: tuple[int, ...], dtyp
 
 def _apart(t: torch.Tensor, what: str) -> None:
     """An output whose elements share no memory (an expanded tensor's do)."""
+    if t.is_contiguous():
+        return
     need = 1
     for stride, size in sorted(zip(t.stride(), t.shape)):
         if size > 1:
