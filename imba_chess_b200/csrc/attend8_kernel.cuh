@@ -16,9 +16,10 @@
 // and not sixteen: a decode step has few of them, and every instruction but
 // the conversions is per row.  The weights pass from the result's layout to the
 // operand's by movmatrix.  A step of 1,024 one-token games (8 heads of 64)
-// takes 35 us, 1.7 TB/s, of which the chain of dependent loads and the plan
-// are the most; 32 long sequences (8 heads of 128, four query heads each)
-// 263 us, 4.9 TB/s.  With the rows as the 16-row operand they took 45 and 324.
+// takes 34 us, 1.8 TB/s, of which the chain of dependent loads is the most (and
+// 104 bytes a thread of spills at three CTAs' 80 registers); 32 long sequences
+// (8 heads of 128, four query heads each) 263 us, 4.9 TB/s.  With the rows as
+// the 16-row operand they took 45 and 324.
 //
 // A contraction may run over its dimension in any order as long as both
 // operands agree, so the order is chosen for the loads: a lane reads 16 (8
@@ -29,13 +30,16 @@
 // the cp.async ring in shared memory needs no barrier.
 //
 // Numerics.  A query row is divided by the power of two of its largest
-// element before it becomes f16 (bf16 queries lose nothing above 2^-24 of
-// that element; fp32 queries are the sum of two f16 parts, 22 bits).  Weights
-// are held relative to a running maximum that is raised when a score passes
-// it by 2^kSlack, times 2^kShift so that small ones stay normal in f16 (fp32:
-// two parts); V's scale enters as its ratio to a reference exponent that
-// follows the blocks (|log2 ratio| <= kVWindow, else the sums so far are
-// rescaled, a power of two).  Sums, maxima and weights are fp32.
+// element before it becomes f16 (bf16 queries are exact down to 2^-17 of that
+// element and off by 2^-25 of it at most below; fp32 queries are the sum of two
+// f16 parts, 22 bits, off by 2^-25 of it at most too).  Weights are held
+// relative to a running maximum that is raised when a score passes it by
+// 2^kSlack, times 2^kShift so that small ones stay normal in f16 (fp32: two
+// parts); one below 2^-30 of the row's largest counts in the sum alone.  V's
+// scale enters as its ratio to a reference exponent that follows the blocks
+// (|log2 ratio| <= kVWindow, else the sums so far are rescaled, a power of two;
+// a block whose scale is below 2^-80 of the largest so far loses precision, and
+// counts as zero below 2^-110).  Sums, maxima and weights are fp32.
 #pragma once
 
 #include "attend8_common.cuh"

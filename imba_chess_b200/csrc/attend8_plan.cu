@@ -212,8 +212,9 @@ __global__ void attend_rows_kernel(imba_attend_desc r, AttendShape sh, AttendPla
 
 namespace {
 
-// Rows a segment (with its shared heads) from which the tcgen05 kernel's tiles
-// of 128 are better than tiles of 16 by mma.sync.
+// Rows a segment (with its shared heads), on average over the step, from which
+// the tcgen05 kernel's tiles of 128 are better than tiles of 16 by mma.sync.  A
+// model's steps cut their groups into chunks of 64 rows, so theirs stay below.
 // (8 heads of 64, segments of 2k to 12k tokens: 64 rows 99 us against 91, 96
 // rows 98 against 119, 256 rows 160 against 248; heads of 128: 64 rows 180
 // against 139, 96 rows 181 against 191, 256 rows 283 against 422; segments of
@@ -235,10 +236,11 @@ AttendShape shape_of(const imba_cache_desc& c, const imba_attend_desc& r, int rt
   sh.warps = warps;
   sh.min_pages = warps == 1 ? 16 : 8;
   // About four CTAs' worth of units for each that is resident (two of the
-  // tcgen05 kernel's, whose parts are large), but fewer for a step of few
-  // tiles, so that one is not joined from more than about 32 parts: one
-  // sequence of 131,000 tokens (20 rows, 8 heads of 128) takes 80 us as one
-  // wave and 131 as four, 32 long sequences 318 and 260.
+  // tcgen05 kernel's, whose parts are large), but no more than 32 units a tile
+  // and head where that leaves one wave at least, since a tile's parts are
+  // joined by one CTA: one sequence of 131,000 tokens (20 rows, 8 heads of 128)
+  // takes 80 us as one wave and 131 as four, 32 long sequences 318 and 260.
+  // (A wave of few heads can be more parts; most_parts bounds those.)
   const int ctas = std::min(attend8_ctas(c.attention_dim, rt), 2);
   const int64_t few = std::max<int64_t>((flat + sh.tile_rows - 1) / sh.tile_rows, r.num_segs) * c.num_heads * 32;
   const int waves = sh.waves = (int)std::min<int64_t>(rt == kTileGroups ? 2 : 4, std::max<int64_t>(1, few / (148 * ctas)));

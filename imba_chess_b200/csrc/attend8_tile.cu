@@ -17,17 +17,19 @@
 // weights' exponent.
 //
 // What bounds it: the chain of a block, S to maxima to weights to P to P V
-// (some 4,000 cycles a block of a CTA), so two CTAs share an SM (64-key blocks, 256 TMEM columns, 82 KB at head size 64).
+// (some 4,000 cycles a block of a CTA), so two CTAs share an SM (64-key blocks,
+// 256 TMEM columns, 82 KB and, spilling 72 bytes, 80 registers at head size 64).
 // 4 x 512 rows of 16 heads of 64 over 2k to 8k tokens take 179 us, 0.2 PFLOP/s;
 // with one thread a row and all 64 keys 215, two stages of K and V 205, a
 // fourth page warp apart from the products' lane 194, and tiles of 16 rows by
 // mma.sync 280.
 //
-// Numerics as in the mma.sync kernel (attend8_kernel.cuh), but that ordinary
-// scores without a bias become weights in one fused step, which the rounding of
-// kShift - maximum puts off by 2^-8 of a unit of log2 at most, all alike.  V's scales of a
-// block's four pages are held against one reference; where they lie more than
-// 2^kSpread apart, the block's P V is done page by page.
+// Numerics as in the mma.sync kernel (attend8_kernel.cuh), but that scores
+// without a bias become weights in one fused step while the row's maximum is
+// within kNear: the rounding of kShift - maximum puts them off by 2^-8 of a unit
+// of log2 at most there, all keys of a maximum alike.  V's scales of a block's
+// four pages are held against one reference; where they lie more than 2^kSpread
+// apart, the block's P V is done page by page.
 #include <algorithm>
 
 #include "attend8_common.cuh"

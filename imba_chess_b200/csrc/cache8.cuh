@@ -69,7 +69,7 @@ __device__ __forceinline__ int scale_byte(float amax) {
 }
 // 2^(b - 127); 0 for an empty block.
 __device__ __forceinline__ float scale_of(int b) { return __uint_as_float((uint32_t)b << 23); }
-// 2^(127 - b) for a scale byte b >= kMinScaleByte (b <= 246: amax is finite).
+// 2^(127 - b) for a scale byte b >= kMinScaleByte (b <= 247: amax is finite).
 __device__ __forceinline__ float inv_scale_of(int b) { return __uint_as_float((uint32_t)(254 - b) << 23); }
 
 // Two floats to two e4m3 codes, rounded to nearest even (lo in the low byte).

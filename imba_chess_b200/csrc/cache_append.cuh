@@ -23,8 +23,9 @@
 // What bounds it: for documents the bytes (1.2 GB of four documents, 8 heads of
 // 128 and 32 query heads, in 254 us, 4.8 TB/s; the rotation and the codes hide
 // behind the loads of the next block), for prefixes of many games the pages'
-// turns and codes as well (57k tokens of 8 heads of 64, 85 us, 3.1 TB/s), for a
-// decode step the launch (1,024 tokens 4.4 us, one token 2.8).
+// turns and codes as well (52k tokens of 8 heads of 64, 85 us, 3.1 TB/s; the
+// kernel of that size spills 180 bytes a thread at its 80 registers), for a
+// decode step the launch (1,024 tokens 4.3 us, one token 2.8).
 #pragma once
 
 #include <algorithm>
@@ -933,7 +934,7 @@ imba_status_t launch_append(const imba_cache_desc& c, const imba_pool_desc& pool
   // Fast: runs of eight elements by 16-byte accesses.  A rotation whose halves
   // are no multiple of eight cuts runs in two, and rows that are not contiguous
   // or aligned have none: these go by single elements (8 heads of 64 as fast
-  // rows, 57k tokens 85 us; 120k tokens of 2 + 16 heads of 64, 58 of 64 elements
+  // rows, 52k tokens 85 us; 120k tokens of 2 + 16 heads of 64, 58 of 64 elements
   // rotated, 588 us for 585 MB, a sixth of the rate).
   bool fast = d.rotary.rot_dim % 16 == 0;
   fast &= take_strides<T>(d.k_stride, d.k, k_tile, &a.ks);
@@ -946,7 +947,7 @@ imba_status_t launch_append(const imba_cache_desc& c, const imba_pool_desc& pool
   a.status = d.status;
   a.num_slots = pool.num_pages * kTok;
   // A row of few heads is one or two passes of a warp: several rows then keep
-  // its loads in flight (57k rows of 8 heads of 64 84 us with four, 98 with one;
+  // its loads in flight (52k rows of 8 heads of 64 84 us with four, 98 with one;
   // rows of 32 heads of 128 274 and 250), if the SMs stay full.
   a.q_rows = d.num_rows >= 148 * 2 * kWarps * kQueryRows && a.Hq * c.attention_dim <= 1024 ? kQueryRows : 1;
   const int64_t q_blocks = a.Hq ? (d.num_rows + kWarps * a.q_rows - 1) / (kWarps * a.q_rows) : 0;

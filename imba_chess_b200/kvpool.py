@@ -124,8 +124,9 @@ class KVPool:
         the last call) of a pool in 8 bits, on the current stream.  The
         operators and the model's steps call this; a caller that recycles
         pages without ``alloc``, or captures a CUDA graph after one, does.
-        Behind all that the pool's other streams have enqueued (a graph's
-        replays are not known here: order them yourself)."""
+        Behind all that the pool's other streams, which have to live as long
+        as it does, have enqueued (a graph's replays are not known here: order
+        them yourself)."""
         if self.scales is None or (pages is None and not self._fresh):
             return
         if self.data.is_cuda:

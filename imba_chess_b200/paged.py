@@ -21,11 +21,12 @@ and arrays are copied through pinned memory): what only the device can see
 written to ``pool``'s status word and raised by ``check_status(pool)``.
 
 A plan keeps the tensors it was made from and its scratch: calls on one plan
-must not overlap (two streams, two captured graphs), and the plan's tensors
-hold the step's rows as they were when it was made.  A call on another stream
-than the plan's waits for nothing by itself, as with any tensor, and marks the
-plan's memory as used there; a captured graph needs its plans kept alive.  A
-pool in 8 bits orders its streams where it empties pages (``kvpool``).
+must not overlap (two streams, two captured graphs), and int32 tensors that were
+on the device already are used as they are, so leave them as they were when the
+plan was made.  A call on another stream than the plan's waits for nothing by
+itself, as with any tensor, and marks the plan's memory as used there; a captured
+graph needs its plans kept alive.  A pool in 8 bits orders its streams where it
+empties pages (``kvpool``).
 """
 
 from __future__ import annotations

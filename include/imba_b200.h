@@ -381,7 +381,9 @@ IMBA_API imba_status_t imba_kv_read(const imba_cache_desc* cache, const imba_poo
  * group each; row r sees the first row_vis[r] tokens of its group's page
  * list, then its extra keys, as in imba_step_desc; a row that sees nothing
  * gets zeros, and rows of no segment are left as they were.  Query head j
- * reads key / value head j / (num_q_heads / num_heads). */
+ * reads key / value head j / (num_q_heads / num_heads).  Values of blocks whose
+ * scale is below 2^-80 of the largest in the list lose precision, and count as
+ * zero below 2^-110. */
 typedef struct imba_attend_desc {
   int32_t num_rows;
   int32_t num_segs;

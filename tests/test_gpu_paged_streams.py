@@ -145,3 +145,38 @@ def test_host_data_is_copied_when_it_is_given():
     torch.cuda.synchronize()
     paged.check_status(pool)
     del keep
+
+
+@pytest.mark.parametrize("rows", [3, 100])
+def test_calls_at_once(rows):
+    """Two streams, and two graphs, with a plan each, over one pool at the same time."""
+    n, streams = 3000, [torch.cuda.Stream() for _ in range(2)]
+    pool = _pool(pages=200)
+    seq = KVSequence(pool)
+    slots = seq.reserve(n)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    rand = lambda *s: torch.randn(s, dtype=torch.bfloat16, device=DEV, generator=gen)  # noqa: E731
+    paged.kv_append(pool, 0, paged.AppendPlan(pool, slots), rand(n, 2, 64), rand(n, 2, 64))
+    plan = lambda: paged.AttentionPlan(pool, row_off=[0, rows], row_vis=[n - i for i in range(rows)],  # noqa: E731
+                                       page_off=[0, len(seq.pages)], pages=seq.pages, num_q_heads=4)
+    plans, q = [plan(), plan()], [rand(rows, 4, 64) for _ in streams]
+    want = [paged.paged_attention(pool, 0, plans[0], x) for x in q]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(25):
+        for s, p, x, g in zip(streams, plans, q, got):
+            with torch.cuda.stream(s):
+                g.append(paged.paged_attention(pool, 0, p, x))
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in streams], []
+    for graph, p, x in zip(graphs, plans, q):
+        with torch.cuda.graph(graph):
+            outs.append([paged.paged_attention(pool, 0, p, x) for _ in range(5)])
+    for _ in range(5):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    paged.check_status(pool)
+    for w, g, o in zip(want, got, outs):
+        assert all(torch.equal(w, x) for x in g + o)
