@@ -59,7 +59,7 @@ def to_device(host: torch.Tensor, device: torch.device) -> torch.Tensor:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("host data cannot be copied in a capture (its replays would copy it again): "
                                "put it on the device before")
-        pinned = torch.empty(host.shape, dtype=host.dtype, pin_memory=True)
+        pinned = torch.empty(host.shape, dtype=host.dtype, device="cpu", pin_memory=True)
         return pinned.copy_(host).to(device, non_blocking=True)
 
 
@@ -135,7 +135,7 @@ class KVPool:
                     raise RuntimeError("pages are not emptied in a capture: call pool.begin_pages() before the capture")
         if pages is None:
             pages, self._fresh = self._fresh, []
-        ids = torch.as_tensor(pages, dtype=torch.int64).cpu()
+        ids = torch.as_tensor(pages, dtype=torch.int64, device="cpu")
         if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= self.num_pages):
             raise ValueError("begin_pages: page id outside the pool")
         if self.data.is_cuda:

@@ -113,7 +113,7 @@ def _ints(x, pool: KVPool, what: str, shape: tuple[int, ...] | None = None) -> t
     """A contiguous int32 tensor on the pool's device.  Wider integers that are
     on the device already are clamped, not wrapped: what was outside int32 is
     then outside every pool and is reported there."""
-    t = torch.as_tensor(x)
+    t = x if isinstance(x, torch.Tensor) else torch.as_tensor(x, device="cpu")
     if t.numel() and (t.is_floating_point() or t.is_complex() or t.dtype == torch.bool):
         raise ValueError(f"{what} must be integers")
     if t.dtype != torch.int32 and not t.is_cuda and t.numel() and (int(t.max()) > 2**31 - 1 or int(t.min()) < -(2**31)):

@@ -138,3 +138,26 @@ def test_attention_in_place_of_split_lists(dtype):
         q = _rand(rng, (rows + 2, 2, 64), dtype, 0.3)
         want = paged.paged_attention(pool, 0, plan, q)
         assert torch.equal(paged.paged_attention(pool, 0, plan, q, out=q), want)
+
+
+def test_host_data_under_a_default_device():
+    """Lists are host data whatever torch's default device is."""
+    rng = np.random.default_rng(6)
+    pool = _pool(pages=4)
+    k, v, q = (_rand(rng, (3, h, 64)) for h in (2, 2, 2))
+    torch.set_default_device("cuda")
+    try:
+        pool.alloc(2)
+        plan = paged.AppendPlan(pool, [0, 1, 2])
+        paged.kv_append(pool, 0, plan, k, v)
+        sees = paged.AttentionPlan(pool, row_off=[0, 3], row_vis=[1, 2, 3], page_off=[0, 1], pages=[0], num_q_heads=2)
+        got = paged.paged_attention(pool, 0, sees, q)
+        paged.kv_read(pool, 0, [0, 1, 2])
+        pool.begin_pages([3])
+        with pytest.raises(ValueError, match="int32"):
+            paged.AppendPlan(pool, [2**31])
+    finally:
+        torch.set_default_device(None)
+    paged.check_status(pool)
+    sees = paged.AttentionPlan(pool, row_off=[0, 3], row_vis=[1, 2, 3], page_off=[0, 1], pages=[0], num_q_heads=2)
+    assert torch.equal(got, paged.paged_attention(pool, 0, sees, q)) and got.any()
