@@ -75,6 +75,17 @@ class KVPool:
         self.dtype = dtype
         self.device = device
         self.scales: torch.Tensor | None = None
+        with torch.inference_mode(False):  # (pages are emptied in place, in that mode and outside of it)
+            self._make(num_layers, num_heads, attention_dim, linear_dim)
+        self._free = np.arange(self.num_pages - 1, -1, -1, dtype=np.int64).tolist()
+        self._fresh: list[int] = []  # pages in 8 bits handed out since begin_pages()
+        self._streams: dict[int, torch.cuda.Stream] = {}  # that calls on a pool in 8 bits ran on, by handle
+        self._ordered: set[int] = set()  # of them, those behind the last begin_pages()
+        self._begun_on: torch.cuda.Stream | None = None  # where that one ran
+        self.desc = _native.PoolDesc(self.data.data_ptr(), self.num_pages)
+
+    def _make(self, num_layers: int, num_heads: int, attention_dim: int, linear_dim: int) -> None:
+        dtype, device = self.dtype, self.device
         if dtype == torch.float8_e4m3fn:
             dims = (32, 64, 96, 128)
             if attention_dim not in dims or linear_dim not in dims or (
@@ -87,14 +98,8 @@ class KVPool:
             self.scales = memory[codes:].view(self.num_pages, num_layers, 2, num_heads)
         else:
             self.data = torch.zeros((self.num_pages, self.page_elems), dtype=dtype, device=device)
-        self._free = np.arange(self.num_pages - 1, -1, -1, dtype=np.int64).tolist()
-        self._fresh: list[int] = []  # pages in 8 bits handed out since begin_pages()
-        self._streams: dict[int, torch.cuda.Stream] = {}  # that calls on a pool in 8 bits ran on, by handle
-        self._ordered: set[int] = set()  # of them, those behind the last begin_pages()
-        self._begun_on: torch.cuda.Stream | None = None  # where that one ran
         # what the operators on the pool report to (made here: in a capture, each replay would clear it)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
-        self.desc = _native.PoolDesc(self.data.data_ptr(), self.num_pages)
 
     @property
     def free_pages(self) -> int:
