@@ -81,8 +81,14 @@ class KVPool:
         self._fresh: list[int] = []  # pages in 8 bits handed out since begin_pages()
         self._streams: dict[int, torch.cuda.Stream] = {}  # that calls on a pool in 8 bits ran on, by handle
         self._ordered: set[int] = set()  # of them, those behind the last begin_pages()
-        self._begun_on: torch.cuda.Stream | None = None  # where that one ran
+        self._begun_on: torch.cuda.Stream | None = None  # where that one, or at first the making of the pool, ran
+        if self.scales is not None and self.data.is_cuda:
+            self._began(torch.cuda.current_stream(self.data.device))
         self.desc = _native.PoolDesc(self.data.data_ptr(), self.num_pages)
+
+    def _began(self, stream: torch.cuda.Stream) -> None:
+        self._streams[stream.cuda_stream] = self._begun_on = stream
+        self._ordered = {stream.cuda_stream}
 
     def _make(self, num_layers: int, num_heads: int, attention_dim: int, linear_dim: int) -> None:
         dtype, device = self.dtype, self.device
@@ -145,18 +151,16 @@ class KVPool:
             raise ValueError("begin_pages: page id outside the pool")
         if self.data.is_cuda:
             stream = torch.cuda.current_stream(self.data.device)
-            self._streams[stream.cuda_stream] = stream
             for other in self._streams.values():
                 if other.cuda_stream != stream.cuda_stream:
                     stream.wait_stream(other)
-            self._ordered = {stream.cuda_stream}
-            self._begun_on = stream
+            self._began(stream)
         self.scales.index_fill_(0, to_device(ids, self.data.device), 0)
 
     def join_stream(self) -> None:
         """The current stream is one that works on this pool in 8 bits: its
-        next work comes after the last ``begin_pages``, and the next
-        ``begin_pages`` after its work."""
+        next work comes after the last ``begin_pages`` (at first, after the
+        making of the pool), and the next ``begin_pages`` after its work."""
         stream = torch.cuda.current_stream(self.data.device)
         with torch.cuda.device(self.data.device):
             if torch.cuda.is_current_stream_capturing():

@@ -180,3 +180,23 @@ def test_calls_at_once(rows):
     paged.check_status(pool)
     for w, g, o in zip(want, got, outs):
         assert all(torch.equal(w, x) for x in g + o)
+
+
+def test_a_new_pool_on_another_stream():
+    """A pool that is still being cleared on the stream it was made on."""
+    warm, ready = _pool(pages=4), torch.cuda.Stream()
+    _, plan, kv, q, sees = _step(warm, 10, 1)
+    paged.kv_append(warm, 0, plan, *kv)
+    want = paged.kv_read(warm, 0, plan.slots)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda._sleep(LONG)
+        pool = _pool(pages=4)
+    with torch.cuda.stream(ready):
+        paged.kv_append(pool, 0, paged.AppendPlan(pool, plan.slots), *kv)
+        got = paged.kv_read(pool, 0, plan.slots)
+    torch.cuda.synchronize()
+    paged.check_status(pool)
+    late = paged.kv_read(pool, 0, plan.slots)
+    for w, g, l in zip(want, got, late):
+        assert torch.equal(w, g) and torch.equal(w, l)
