@@ -239,7 +239,8 @@ def kv_append(pool: KVPool, layer: int, plan: AppendPlan, k: torch.Tensor, v: to
         else:
             _rows(q_out, pool, "q_out", q.shape, dtype)
             _apart(q_out, "q_out")
-            if q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride():
+            if q_out.data_ptr() == q.data_ptr() and any(
+                    a != b for a, b, size in zip(q.stride(), q_out.stride(), q.shape) if size > 1):
                 raise ValueError("q_out overlaps q in another order")
         if q.numel():
             q_heads, q_ptrs, q_strides = q.shape[1], (q.data_ptr(), q_out.data_ptr()), (*q.stride(), *q_out.stride())

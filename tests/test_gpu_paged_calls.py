@@ -110,6 +110,8 @@ def test_outputs_that_share_memory():
     assert torch.equal(paged.kv_append(pool, 0, plan, k, v, q=q, q_out=odd), q)
     tight = torch.zeros(4 * 265, dtype=torch.bfloat16, device=DEV).as_strided((4, 4, 64), (265, 67, 1))
     assert torch.equal(paged.kv_append(pool, 0, plan, k, v, q=q, q_out=tight), q)
+    first = q[:1].as_strided((1, 4, 64), (7, 64, 1))  # a row alone has any stride
+    assert paged.kv_append(pool, 0, paged.AppendPlan(pool, [8]), k[:1], v[:1], q=q[:1], q_out=first) is first
     one = base[:256].view(1, 4, 64)[:, :1].expand(1, 1, 64)
     assert paged.kv_append(pool, 0, paged.AppendPlan(pool, [9]), k[:1], v[:1], q=q[:1, :1], q_out=one) is one
     for rows in (4, 90):  # both kernels
